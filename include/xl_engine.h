@@ -348,6 +348,104 @@ XL_API int xl_op_embedding(const float* table, const int* ids, float* out, int n
 XL_API int xl_op_attn_prefill(float* qkv, const float* rope, float* kc, float* vc, float* out, int n, int heads,
                               int max_ctx, void* stream);
 
+/* ---- 8-bit projections and a paged key/value cache (no reference counterpart) ----
+ * The pieces of a decoder layer's serving step with e4m3 weights and
+ * activations, for several sequences of unlike lengths:
+ *
+ *   xl_op_add_rmsnorm_fp8 -> xl_op_linear_fp8 (QKV) -> xl_op_attn_decode_paged
+ *   -> xl_op_quantize_fp8 -> xl_op_linear_fp8 (out-projection)
+ *   -> xl_op_add_rmsnorm_fp8 -> xl_op_linear_fp8 (W1/V, SwiGLU)
+ *   -> xl_op_quantize_fp8 -> xl_op_linear_fp8 (W2)
+ *
+ * Common to them: matrices are row-major; `dtype` is the element type of the
+ * rows (XL_F32, XL_BF16, XL_F16); device pointers belong to the current
+ * device, the stream too (a pointer of another device, or of the host, is
+ * refused with XL_ERR_ARG); matrix and row pointers are 16-byte aligned, every
+ * other pointer aligned to its element, NULL only where said; each call is one
+ * kernel, asynchronous on `stream`, allocates nothing, and may be captured
+ * into a graph.  Inputs and outputs do not overlap except where said.
+ *
+ * An e4m3 matrix [n][k] has rows of ldq bytes (a multiple of 16, at least k)
+ * and a float scale for each group of 128 columns: scale is
+ * [n][ceil(k / 128)] for activations (one row a scale) and
+ * [ceil(n / 128)][ceil(k / 128)] for weights (128 rows a scale); a value is
+ * q * scale.  Bytes from k to ldq are neither read nor written. */
+enum { XL_F32 = 0, XL_BF16 = 1, XL_F16 = 2 };
+
+/* q, scale from x [n][k] (rows of ldx elements, any ldx >= k; x itself may be
+ * aligned to its element only), per group with
+ * a = max |x|: scale = a / 448 in fp32, q = x / scale rounded to nearest, ties
+ * to even.  A group of zeros has scale 0 and q 0; a group with a value that is
+ * not finite has scale NaN and q NaN.  rows_per_scale: 1 or 128.
+ * ceil(n / rows_per_scale) * ceil(k / 128) <= 2^31 - 1. */
+XL_API int xl_op_quantize_fp8(int dtype, const void* x, size_t ldx, uint8_t* q, size_t ldq, float* scale, int n, int k,
+                              int rows_per_scale, void* stream);
+
+/* r = residual + delta rounded to dtype and stored in residual_out (which may
+ * be residual itself); then r's RMSNorm (eps 1e-6, gain gamma[k]) as e4m3 rows
+ * with one scale per row and 128 columns, as xl_op_quantize_fp8 makes them of
+ * unrounded values.  delta may be NULL: r is residual and nothing is stored
+ * (residual_out is not used).  residual, delta and residual_out are [n][k] of
+ * dtype; k <= 32768. */
+XL_API int xl_op_add_rmsnorm_fp8(int dtype, const void* delta, const void* residual, void* residual_out,
+                                 const float* gamma, uint8_t* q, size_t ldq, float* scale, int n, int k, void* stream);
+
+/* y = x . w^T + bias from e4m3 operands: xq [n][k] with x_scale
+ * [n][ceil(k / 128)], wq [m][k] with w_scale [ceil(m / 128)][ceil(k / 128)];
+ * sums in fp32.  The modes of xl_op_linear: 0 y [n][m]; 1 SwiGLU over
+ * interleaved (W1, V) rows, y [n][m / 2], m even; 2 y [n][m] += .  dtype is
+ * y's type; bias [m] may be NULL. */
+XL_API int xl_op_linear_fp8(int mode, int dtype, const uint8_t* xq, size_t ldx, const float* x_scale, const uint8_t* wq,
+                            size_t ldw, const float* w_scale, const float* bias, void* y, int n, int m, int k,
+                            void* stream);
+
+/* A paged cache: pools k and v [num_pages][kv_heads][page_size][head_dim] of
+ * dtype; page_table [batch][max_pages] (device ints) names the pages of each
+ * sequence in order.  head_dim 64 or 128; max_pages * page_size <= 2^31 - 1.
+ * Entries past the pages that a sequence's positions need are not read.
+ * Sequences may share pages that are not written any more.  The struct itself
+ * is host memory, read during the call only. */
+typedef struct xl_paged_kv {
+    void* k;
+    void* v;
+    const int* page_table;
+    int dtype;
+    int batch;
+    int kv_heads;
+    int head_dim;
+    int page_size;
+    int max_pages;
+    int num_pages;
+} xl_paged_kv;
+
+/* Keys and values of `rows` rows (prompts) into their pages: row i of qkv
+ * ([rows][(heads + 2 kv_heads) head_dim], q | k | v) goes to position
+ * row_pos[i] of sequence row_seq[i] (device ints), its key rotated by the
+ * angles rope[row_pos[i]] ([rope_len][head_dim / 2] pairs of cos and sin:
+ * xl_rope_table for head_dim 64) or as it is where rope is NULL.  A row whose
+ * sequence, position or page is out of range is skipped; positions past
+ * rope_len are out of range.  Two rows for one position: either is stored. */
+XL_API int xl_op_kv_append_paged(const xl_paged_kv* cache, int dtype, const void* qkv, const float* rope, int rope_len,
+                                 const int* row_seq, const int* row_pos, int rows, int heads, void* stream);
+
+/* xl_op_attn_decode over a paged cache, for cache->batch sequences: the new
+ * token of sequence b (row b of qkv, as above) has position pos[b] (device
+ * int); its key (rotated) and value are stored there, and out [batch][heads *
+ * head_dim] is the attention of its rotated query over positions 0 .. pos[b]
+ * as the cache holds them (scale head_dim^-1/2).  heads is a multiple of
+ * kv_heads; query head h reads key/value head h / (heads / kv_heads).
+ * pos[b] = -1: no sequence, zeros.  Any other position out of range, or a page
+ * id outside [0, num_pages) among the pages needed: NaN outputs for that
+ * sequence, and nothing is read or written through that position or page.
+ * workspace: xl_op_attn_decode_paged_workspace_bytes(cache, heads) bytes,
+ * zero-filled before first use (left ready for the next call, whatever its
+ * shape, on the same stream); calls that may run at the same time, replayed
+ * graphs too, need workspaces of their own. */
+XL_API size_t xl_op_attn_decode_paged_workspace_bytes(const xl_paged_kv* cache, int heads);
+XL_API int xl_op_attn_decode_paged(const xl_paged_kv* cache, int dtype, const void* qkv, const float* rope, int rope_len,
+                                   const int* pos, void* out, int heads, void* workspace, size_t workspace_bytes,
+                                   void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -25,7 +25,22 @@ _SIGS = {
     "xl_op_rmsnorm": ([VP, VP, VP, I, I, VP], I),
     "xl_op_embedding": ([VP, VP, VP, I, I, VP], I),
     "xl_op_attn_prefill": ([VP, VP, VP, VP, VP, I, I, I, VP], I),
+    "xl_op_quantize_fp8": ([I, VP, SZ, VP, SZ, VP, I, I, I, VP], I),
+    "xl_op_add_rmsnorm_fp8": ([I, VP, VP, VP, VP, VP, SZ, VP, I, I, VP], I),
+    "xl_op_linear_fp8": ([I, I, VP, SZ, VP, VP, SZ, VP, VP, VP, I, I, I, VP], I),
+    "xl_op_kv_append_paged": ([VP, I, VP, VP, I, VP, VP, I, I, VP], I),
+    "xl_op_attn_decode_paged_workspace_bytes": ([VP, I], SZ),
+    "xl_op_attn_decode_paged": ([VP, I, VP, VP, I, VP, VP, I, VP, SZ, VP], I),
 }
+
+XL_F32, XL_BF16, XL_F16 = 0, 1, 2
+
+
+class PagedKV(C.Structure):
+    """xl_paged_kv of include/xl_engine.h."""
+    _fields_ = [(n, VP) for n in ("k", "v", "page_table")] + \
+               [(n, I) for n in ("dtype", "batch", "kv_heads", "head_dim", "page_size", "max_pages", "num_pages")]
+
 
 _lib = None
 

@@ -2,10 +2,12 @@
 #include <nccl.h>
 
 #include <cstring>
+#include <initializer_list>
 #include <string>
 #include <vector>
 
 #include "engine.h"
+#include "paged.h"
 
 using xl::Engine;
 
@@ -457,6 +459,170 @@ int xl_op_attn_prefill(float* qkv, const float* rope, float* kc, float* vc, floa
     int rc = cuda_status(xl::launch_rope_kv_prefill(qkv, r2, kc, vc, n, heads, max_ctx, s), "rope_kv_prefill");
     if (rc != XL_OK) return rc;
     return cuda_status(xl::launch_attn_prefill(qkv, kc, vc, out, nullptr, n, heads, max_ctx, s), "attn_prefill");
+}
+
+// ---- 8-bit projections and the paged cache ----
+namespace {
+
+bool aligned(const void* p, size_t to) { return reinterpret_cast<uintptr_t>(p) % to == 0; }
+
+size_t type_bytes(int dtype) { return dtype == xl::kF32 ? 4 : 2; }
+bool type_ok(int dtype) { return dtype == xl::kF32 || dtype == xl::kBF16 || dtype == xl::kF16; }
+
+// Each pointer (null ones aside) has to be memory of the current device, whose
+// SM count goes to *sms: a kernel given another device's or the host's memory
+// would fault.
+int on_current_device(const char* what, std::initializer_list<const void*> ptrs, int* sms) {
+    int dev = 0;
+    int rc = cuda_status(cudaGetDevice(&dev), what);
+    if (rc != XL_OK) return rc;
+    for (const void* p : ptrs) {
+        if (!p) continue;
+        cudaPointerAttributes a{};
+        const cudaError_t e = cudaPointerGetAttributes(&a, p);
+        if (e != cudaSuccess) {
+            cudaGetLastError();
+            return cuda_status(e, what);
+        }
+        if (a.type != cudaMemoryTypeManaged && (a.type != cudaMemoryTypeDevice || a.device != dev)) {
+            xl::set_error(std::string(what) + ": a pointer is not memory of the current device");
+            return XL_ERR_ARG;
+        }
+    }
+    return cuda_status(cudaDeviceGetAttribute(sms, cudaDevAttrMultiProcessorCount, dev), what);
+}
+
+// Null if the cache's description is in order, else what is wrong with it.
+const char* paged_fault(const xl_paged_kv* c, int heads) {
+    if (!c || !c->k || !c->v || !c->page_table) return "null pointer";
+    if (!type_ok(c->dtype)) return "unknown cache dtype";
+    if (c->batch <= 0 || c->kv_heads <= 0 || c->page_size <= 0 || c->max_pages <= 0 || c->num_pages <= 0 || heads <= 0)
+        return "sizes must be positive";
+    if (c->head_dim != 64 && c->head_dim != 128) return "head_dim must be 64 or 128";
+    if (heads % c->kv_heads) return "heads must be a multiple of kv_heads";
+    if (static_cast<long long>(c->max_pages) * c->page_size > 0x7fffffffll) return "max_pages * page_size is over 2^31 - 1";
+    if (static_cast<long long>(c->batch) * heads > 0x3fffffffll) return "batch * heads is over 2^30 - 1";
+    if (!aligned(c->k, 16) || !aligned(c->v, 16) || !aligned(c->page_table, 4)) return "cache pointers must be 16-byte aligned";
+    return nullptr;
+}
+
+xl::PagedCache paged_of(const xl_paged_kv& c) {
+    return {c.k, c.v, c.page_table, c.dtype, c.batch, c.kv_heads, c.head_dim, c.page_size, c.max_pages, c.num_pages};
+}
+
+int bad_op(const char* op, const char* why) {
+    xl::set_error(std::string(op) + ": " + why);
+    return XL_ERR_ARG;
+}
+
+}  // namespace
+
+int xl_op_quantize_fp8(int dtype, const void* x, size_t ldx, uint8_t* q, size_t ldq, float* scale, int n, int k,
+                       int rows_per_scale, void* stream) {
+    static const char op[] = "xl_op_quantize_fp8";
+    xl::clear_error();
+    if (!x || !q || !scale) return bad_op(op, "null pointer");
+    if (!type_ok(dtype)) return bad_op(op, "unknown dtype");
+    if (n <= 0 || k <= 0) return bad_op(op, "n and k must be positive");
+    if (rows_per_scale != 1 && rows_per_scale != xl::kFp8Block) return bad_op(op, "rows_per_scale must be 1 or 128");
+    if (ldx < static_cast<size_t>(k)) return bad_op(op, "ldx must be at least k");
+    if (ldq < static_cast<size_t>(k) || ldq % 16 || !aligned(q, 16))
+        return bad_op(op, "q must be 16-byte aligned, with rows of ldq >= k bytes, a multiple of 16");
+    if (!aligned(x, type_bytes(dtype)) || !aligned(scale, 4)) return bad_op(op, "a pointer is not aligned to its element");
+    const long long groups = (static_cast<long long>(n) + rows_per_scale - 1) / rows_per_scale *
+                             ((k - 1) / xl::kFp8Block + 1);
+    if (groups > 0x7fffffffll) return bad_op(op, "too many groups");
+    int sms = 0;
+    const int rc = on_current_device(op, {x, q, scale}, &sms);
+    if (rc != XL_OK) return rc;
+    return cuda_status(
+        xl::launch_quantize_fp8(dtype, x, ldx, q, ldq, scale, n, k, rows_per_scale, sms, as_stream(stream)), op);
+}
+
+int xl_op_add_rmsnorm_fp8(int dtype, const void* delta, const void* residual, void* residual_out, const float* gamma,
+                          uint8_t* q, size_t ldq, float* scale, int n, int k, void* stream) {
+    static const char op[] = "xl_op_add_rmsnorm_fp8";
+    xl::clear_error();
+    if (!residual || !gamma || !q || !scale) return bad_op(op, "null pointer");
+    if (delta && !residual_out) return bad_op(op, "residual_out is missing");
+    if (!type_ok(dtype)) return bad_op(op, "unknown dtype");
+    if (n <= 0 || k <= 0 || k > xl::kNormMaxK) return bad_op(op, "n must be positive and k in [1, 32768]");
+    if (ldq < static_cast<size_t>(k) || ldq % 16 || !aligned(q, 16))
+        return bad_op(op, "q must be 16-byte aligned, with rows of ldq >= k bytes, a multiple of 16");
+    if (!aligned(residual, 16) || !aligned(delta, 16) || (delta && !aligned(residual_out, 16)) || !aligned(gamma, 16) ||
+        !aligned(scale, 4))
+        return bad_op(op, "residual, delta, residual_out and gamma must be 16-byte aligned");
+    if (delta && delta == residual_out) return bad_op(op, "residual_out must not be delta");
+    int sms = 0;
+    const int rc = on_current_device(op, {delta, residual, delta ? residual_out : nullptr, gamma, q, scale}, &sms);
+    if (rc != XL_OK) return rc;
+    return cuda_status(xl::launch_add_rmsnorm_fp8(dtype, delta, residual, residual_out, gamma, q, ldq, scale, n, k,
+                                                  as_stream(stream)), op);
+}
+
+int xl_op_linear_fp8(int mode, int dtype, const uint8_t* xq, size_t ldx, const float* x_scale, const uint8_t* wq,
+                     size_t ldw, const float* w_scale, const float* bias, void* y, int n, int m, int k, void* stream) {
+    static const char op[] = "xl_op_linear_fp8";
+    xl::clear_error();
+    if (!xq || !x_scale || !wq || !w_scale || !y) return bad_op(op, "null pointer");
+    if (mode != xl::kGemvPlain && mode != xl::kGemvSwiGLU && mode != xl::kGemvResidual)
+        return bad_op(op, "mode must be 0, 1 or 2");
+    if (!type_ok(dtype)) return bad_op(op, "unknown dtype");
+    if (n <= 0 || m <= 0 || k <= 0) return bad_op(op, "n, m and k must be positive");
+    if (mode == xl::kGemvSwiGLU && m % 2) return bad_op(op, "SwiGLU needs an even m");
+    if (ldx < static_cast<size_t>(k) || ldw < static_cast<size_t>(k) || ldx % 16 || ldw % 16 || !aligned(xq, 16) ||
+        !aligned(wq, 16))
+        return bad_op(op, "xq and wq must be 16-byte aligned, with rows of at least k bytes, a multiple of 16");
+    if (!aligned(y, 16) || !aligned(x_scale, 4) || !aligned(w_scale, 4) || !aligned(bias, 4))
+        return bad_op(op, "y must be 16-byte aligned, scales and bias 4-byte");
+    int sms = 0;
+    const int rc = on_current_device(op, {xq, x_scale, wq, w_scale, bias, y}, &sms);
+    if (rc != XL_OK) return rc;
+    return cuda_status(xl::launch_linear_fp8(mode, dtype, xq, ldx, x_scale, wq, ldw, w_scale, bias, y, n, m, k, sms,
+                                             as_stream(stream)), op);
+}
+
+int xl_op_kv_append_paged(const xl_paged_kv* cache, int dtype, const void* qkv, const float* rope, int rope_len,
+                          const int* row_seq, const int* row_pos, int rows, int heads, void* stream) {
+    static const char op[] = "xl_op_kv_append_paged";
+    xl::clear_error();
+    if (const char* why = paged_fault(cache, heads)) return bad_op(op, why);
+    if (!qkv || !row_seq || !row_pos) return bad_op(op, "null pointer");
+    if (!type_ok(dtype)) return bad_op(op, "unknown dtype");
+    if (rows <= 0) return bad_op(op, "rows must be positive");
+    if (rope && rope_len <= 0) return bad_op(op, "rope_len must be positive");
+    if (!aligned(qkv, 16) || !aligned(rope, 16) || !aligned(row_seq, 4) || !aligned(row_pos, 4))
+        return bad_op(op, "qkv and rope must be 16-byte aligned");
+    int sms = 0;
+    const int rc = on_current_device(op, {cache->k, cache->v, cache->page_table, qkv, rope, row_seq, row_pos}, &sms);
+    if (rc != XL_OK) return rc;
+    return cuda_status(xl::launch_kv_append_paged(paged_of(*cache), dtype, qkv, rope, rope_len, row_seq, row_pos, rows,
+                                                  heads, as_stream(stream)), op);
+}
+
+size_t xl_op_attn_decode_paged_workspace_bytes(const xl_paged_kv* cache, int heads) {
+    if (paged_fault(cache, heads)) return 0;
+    return xl::attn_paged_ws_bytes(cache->batch, heads, cache->kv_heads);
+}
+
+int xl_op_attn_decode_paged(const xl_paged_kv* cache, int dtype, const void* qkv, const float* rope, int rope_len,
+                            const int* pos, void* out, int heads, void* workspace, size_t workspace_bytes,
+                            void* stream) {
+    static const char op[] = "xl_op_attn_decode_paged";
+    xl::clear_error();
+    if (const char* why = paged_fault(cache, heads)) return bad_op(op, why);
+    if (!qkv || !pos || !out || !workspace) return bad_op(op, "null pointer");
+    if (!type_ok(dtype)) return bad_op(op, "unknown dtype");
+    if (rope && rope_len <= 0) return bad_op(op, "rope_len must be positive");
+    if (!aligned(qkv, 16) || !aligned(rope, 16) || !aligned(out, 16) || !aligned(workspace, 16) || !aligned(pos, 4))
+        return bad_op(op, "qkv, rope, out and workspace must be 16-byte aligned");
+    if (workspace_bytes < xl::attn_paged_ws_bytes(cache->batch, heads, cache->kv_heads))
+        return bad_op(op, "the workspace is too small (xl_op_attn_decode_paged_workspace_bytes)");
+    int sms = 0;
+    const int rc = on_current_device(op, {cache->k, cache->v, cache->page_table, qkv, rope, pos, out, workspace}, &sms);
+    if (rc != XL_OK) return rc;
+    return cuda_status(xl::launch_attn_decode_paged(paged_of(*cache), dtype, qkv, rope, rope_len, pos, out, heads,
+                                                    workspace, sms, as_stream(stream)), op);
 }
 
 }  // extern "C"

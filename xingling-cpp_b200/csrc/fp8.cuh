@@ -1,0 +1,114 @@
+// e4m3 rounding and typed 8-element accesses of the 8-bit serving operators.
+#pragma once
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+#include "xl_kernels.h"
+
+namespace xl {
+
+constexpr float kFp8Max = 448.0f;    // largest e4m3 value
+constexpr uint8_t kFp8NaN = 0x7f;
+
+__device__ __forceinline__ float to_float(float v) { return v; }
+__device__ __forceinline__ float to_float(__nv_bfloat16 v) { return __bfloat162float(v); }
+__device__ __forceinline__ float to_float(__half v) { return __half2float(v); }
+template <typename T>
+__device__ __forceinline__ T from_float(float v);
+template <>
+__device__ __forceinline__ float from_float<float>(float v) { return v; }
+template <>
+__device__ __forceinline__ __nv_bfloat16 from_float<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
+template <>
+__device__ __forceinline__ __half from_float<__half>(float v) { return __float2half_rn(v); }
+
+// 8 consecutive elements of a 16-byte aligned address, as floats.
+template <typename T>
+__device__ __forceinline__ void load8(const T* p, float (&v)[8]) {
+    if constexpr (sizeof(T) == 4) {
+        const float4 a = reinterpret_cast<const float4*>(p)[0], b = reinterpret_cast<const float4*>(p)[1];
+        v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
+    } else {
+        const uint4 u = *reinterpret_cast<const uint4*>(p);
+        const T* e = reinterpret_cast<const T*>(&u);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = to_float(e[i]);
+    }
+}
+template <typename T>
+__device__ __forceinline__ void store8(T* p, const float (&v)[8]) {
+    if constexpr (sizeof(T) == 4) {
+        reinterpret_cast<float4*>(p)[0] = make_float4(v[0], v[1], v[2], v[3]);
+        reinterpret_cast<float4*>(p)[1] = make_float4(v[4], v[5], v[6], v[7]);
+    } else {
+        uint4 u;
+        T* e = reinterpret_cast<T*>(&u);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) e[i] = from_float<T>(v[i]);
+        *reinterpret_cast<uint4*>(p) = u;
+    }
+}
+// The first `live` of 8 consecutive elements (0 for the others); `vec`: the address is 16-byte aligned.
+template <typename T>
+__device__ __forceinline__ void load8_ragged(const T* p, int live, bool vec, float (&v)[8]) {
+    if (vec && live >= 8) {
+        load8(p, v);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = i < live ? to_float(p[i]) : 0.0f;
+    }
+}
+
+// Two floats to two e4m3 bytes (the first in the low byte), to nearest, ties to even; NaN stays NaN.
+__device__ __forceinline__ uint32_t e4m3x2(float lo, float hi) {
+    uint16_t r;
+    asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(r) : "f"(hi), "f"(lo));
+    return r;
+}
+
+// The e4m3 value nearest to v, in one rounding: v goes to 32 bits rounded to
+// odd (truncated, the last bit set where anything was cut), which keeps it on
+// its side of every e4m3 border, and then to 8 bits.
+__device__ __forceinline__ uint32_t e4m3_of(double v) {
+    float f = __double2float_rz(v);
+    if (static_cast<double>(f) != v) f = __uint_as_float(__float_as_uint(f) | 1u);
+    return e4m3x2(f, 0.0f) & 0xffu;
+}
+
+// Whether a 32-bit quotient that is at most 8 units in the last place off may
+// lie on the other side of a border between two e4m3 values than the exact
+// one does.  Borders are where the 4th bit after the leading one is set and
+// nothing follows; below 2^-6 (steps of 2^-9) the odd multiples of 2^-10.
+__device__ __forceinline__ bool near_border(float q) {
+    const uint32_t u = __float_as_uint(q) & 0x7fffffffu;
+    if (u >= 0x3c800000u) return ((u - 0x7fff8u) & 0xfffffu) <= 16u;
+    const float m = __uint_as_float(u) * 1024.0f, r = rintf(m);
+    return fabsf(m - r) < 1e-5f && (static_cast<int>(r) & 1);
+}
+
+// n / d for 0 <= n < 2^31 with a multiplication (Granlund and Montgomery,
+// "Division by invariant integers using multiplication", PLDI 1994): with
+// l = ceil(log2 d) and mul = floor(2^32 (2^l - d) / d) + 1 the quotient is
+// (hi + (n - hi) / 2) >> (l - 1), hi the high word of n * mul.
+struct FastDiv {
+    uint32_t d, mul, shift;
+    FastDiv() = default;
+    explicit FastDiv(uint32_t div) : d(div) {
+        uint32_t l = 0;
+        while ((1ull << l) < div) ++l;
+        mul = static_cast<uint32_t>(((1ull << 32) * ((1ull << l) - div)) / div + 1);
+        shift = l;
+    }
+    __host__ __device__ __forceinline__ uint32_t div(uint32_t n) const {
+#ifdef __CUDA_ARCH__
+        const uint32_t hi = __umulhi(n, mul);
+#else
+        const uint32_t hi = static_cast<uint32_t>((static_cast<uint64_t>(n) * mul) >> 32);
+#endif
+        return shift ? (hi + ((n - hi) >> 1)) >> (shift - 1) : n;
+    }
+};
+
+}  // namespace xl

@@ -1,0 +1,293 @@
+// e4m3 quantisation with a scale per 128 columns, alone (activations: one row
+// a scale; weights: 128 rows a scale) and behind the residual addition and
+// RMSNorm of a sublayer's input.
+//
+//   a = max |y| over the group, s = fl32(a / 448), q = e4m3(y / s)
+//
+// A group of zeros has s = 0 and q = 0; a group that holds a value that is
+// not finite has s = NaN and q = NaN, so what it stands for shows it.
+//
+// The quotients are formed in 32 bits and checked against the borders between
+// e4m3 values; the few that lie next to one are formed again in 64 bits.  So
+// q is the nearest e4m3 value to the exact y / s, whatever the rounding of
+// the fast path, and does not depend on how the work is split.
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include "fp8.cuh"
+#include "xl_device.cuh"
+#include "xl_kernels.h"
+
+namespace xl {
+
+namespace {
+
+constexpr int kLanesPerGroup = 16;  // lanes that share a group: 8 columns each
+constexpr double kNormEps = 1e-6;   // as the engine's RMSNorm
+
+// What divides a group's values: the stored scale and its reciprocal.
+struct GroupScale {
+    float s, inv;
+    bool exact_only;  // the reciprocal overflows (a scale near the smallest floats)
+};
+__device__ __forceinline__ GroupScale group_scale(float s) {
+    GroupScale g;
+    g.s = s;
+    g.exact_only = s > 0.0f && s < 1e-30f;
+    g.inv = s > 0.0f ? 1.0f / s : 0.0f;
+    return g;
+}
+
+// Bytes of 8 quotients; y(i) is the exact value in 64 bits, fast(i) its quotient by the scale in 32.
+template <typename Fast, typename Exact>
+__device__ __forceinline__ uint2 quantise8(const GroupScale& g, Fast fast, Exact y) {
+    float q[8];
+    bool close = g.exact_only;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        q[i] = fast(i);
+        close |= near_border(q[i]);
+    }
+    uint2 out;
+    out.x = e4m3x2(q[0], q[1]) | e4m3x2(q[2], q[3]) << 16;
+    out.y = e4m3x2(q[4], q[5]) | e4m3x2(q[6], q[7]) << 16;
+    if (close && g.s > 0.0f) {
+        out = make_uint2(0u, 0u);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const uint32_t b = e4m3_of(y(i) / static_cast<double>(g.s));
+            if (i < 4) out.x |= b << (8 * i);
+            else out.y |= b << (8 * (i - 4));
+        }
+    }
+    if (!(g.s >= 0.0f)) out.x = out.y = kFp8NaN * 0x01010101u;
+    return out;
+}
+
+__device__ __forceinline__ void store_bytes(uint8_t* p, uint2 b, int live) {
+    if (live >= 8) {
+        *reinterpret_cast<uint2*>(p) = b;
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            if (i < live) p[i] = static_cast<uint8_t>((i < 4 ? b.x : b.y) >> (8 * (i & 3)));
+    }
+}
+
+// Magnitudes compare as unsigned integers, with NaN above infinity.
+__device__ __forceinline__ uint32_t abs_bits(float v) { return __float_as_uint(v) & 0x7fffffffu; }
+__device__ __forceinline__ unsigned long long abs_bits(double v) {
+    return static_cast<unsigned long long>(__double_as_longlong(v)) & 0x7fffffffffffffffull;
+}
+template <typename U>
+__device__ __forceinline__ U umax(U a, U b) { return a > b ? a : b; }
+
+__device__ __forceinline__ float scale_of(uint32_t a) {
+    return a < 0x7f800000u ? __fdiv_rn(__uint_as_float(a), kFp8Max) : __uint_as_float(0x7fffffffu);
+}
+
+template <typename T>
+__device__ __forceinline__ uint2 quantise_plain(const float (&v)[8], const GroupScale& g) {
+    return quantise8(
+        g, [&](int i) { return v[i] * g.inv; }, [&](int i) { return static_cast<double>(v[i]); });
+}
+
+// One scale per row and 128 columns: 16 lanes a group, 8 columns a lane.
+template <typename T>
+__global__ void __launch_bounds__(256) quantize_rows_kernel(const T* __restrict__ x, size_t ldx, uint8_t* __restrict__ q,
+                                                            size_t ldq, float* __restrict__ scale, uint32_t groups,
+                                                            FastDiv per_row, int k, bool vec) {
+    const uint32_t stride = gridDim.x * (256 / kLanesPerGroup);
+    const int sub = threadIdx.x % kLanesPerGroup;
+    // whole warps stay in the loop: the reductions shuffle across the half-warp only, but name the warp
+    const uint32_t first = blockIdx.x * (256 / kLanesPerGroup) + (threadIdx.x / 32) * 2;
+    for (uint32_t base = first; base < groups; base += stride) {
+        const uint32_t gi = base + (threadIdx.x / kLanesPerGroup) % 2;
+        const bool on = gi < groups;
+        const uint32_t row = on ? per_row.div(gi) : 0u;
+        const int c = static_cast<int>(gi - row * per_row.d) * kFp8Block + sub * 8;
+        const int live = on ? max(0, min(8, k - c)) : 0;
+        float v[8];
+        load8_ragged(x + row * ldx + (live ? c : 0), live, vec, v);
+        uint32_t a = 0;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) a = umax(a, abs_bits(v[i]));
+#pragma unroll
+        for (int o = kLanesPerGroup / 2; o; o >>= 1) a = umax(a, __shfl_xor_sync(0xffffffffu, a, o));
+        const GroupScale g = group_scale(scale_of(a));
+        const uint2 b = quantise_plain<T>(v, g);
+        if (live) store_bytes(q + row * ldq + c, b, live);
+        if (on && sub == 0) scale[gi] = g.s;
+    }
+}
+
+// One scale per block of 128 x 128: a CTA keeps the block in registers, so it
+// is read once (64 values a thread, 16 loads of 16 bytes in flight for fp32).
+template <typename T>
+__global__ void __launch_bounds__(256) quantize_blocks_kernel(const T* __restrict__ x, size_t ldx, uint8_t* __restrict__ q,
+                                                              size_t ldq, float* __restrict__ scale, FastDiv per_row,
+                                                              int n, int k, bool vec) {
+    __shared__ uint32_t red[8];
+    const uint32_t rb = per_row.div(blockIdx.x);
+    const int c = static_cast<int>(blockIdx.x - rb * per_row.d) * kFp8Block + (threadIdx.x % kLanesPerGroup) * 8;
+    const int live = max(0, min(8, k - c));
+    const long long r0 = static_cast<long long>(rb) * kFp8Block + threadIdx.x / kLanesPerGroup;
+    float v[8][8];
+    uint32_t a = 0;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+        const long long r = r0 + 16 * j;
+        const bool on = r < n && live;
+        load8_ragged(x + (on ? r * ldx + c : 0), on ? live : 0, vec, v[j]);
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) a = umax(a, abs_bits(v[j][i]));
+#pragma unroll
+    for (int o = 16; o; o >>= 1) a = umax(a, __shfl_xor_sync(0xffffffffu, a, o));
+    if (threadIdx.x % 32 == 0) red[threadIdx.x / 32] = a;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < 8; ++w) a = umax(a, red[w]);
+    const GroupScale g = group_scale(scale_of(a));
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+        const long long r = r0 + 16 * j;
+        if (r < n && live) store_bytes(q + r * ldq + c, quantise_plain<T>(v[j], g), live);
+    }
+    if (threadIdx.x == 0) scale[blockIdx.x] = g.s;
+}
+
+// r = fl_T(residual + delta) (stored where there is a delta), rs =
+// 1 / sqrt(mean(r^2) + eps), y = r gamma rs, e4m3 per row and 128 columns.
+// One row a CTA, kept in registers (CHUNKS x 8 columns a thread), so each
+// input is read once.  The sum of squares and the products r gamma that set
+// the scales are 64-bit: both are exact or nearly so, so a group's scale and
+// bytes do not depend on the order of the sum.
+template <typename T, int CHUNKS>
+__global__ void __launch_bounds__(1024) add_rmsnorm_fp8_kernel(const T* __restrict__ delta, const T* residual, T* sum,
+                                                               const float* __restrict__ gamma, uint8_t* __restrict__ q,
+                                                               size_t ldq, float* __restrict__ scale, int k, bool vec) {
+    __shared__ double red[32];
+    const size_t row = blockIdx.x;
+    const int warp = threadIdx.x >> 5;
+    float r[CHUNKS][8];
+    double ss = 0.0;
+#pragma unroll
+    for (int j = 0; j < CHUNKS; ++j) {
+        const int c = static_cast<int>(threadIdx.x + j * blockDim.x) * 8;
+        const int live = max(0, min(8, k - c));
+        const size_t at = row * k + (live ? c : 0);
+        load8_ragged(residual + at, live, vec, r[j]);
+        if (delta) {
+            float d[8];
+            load8_ragged(delta + at, live, vec, d);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) r[j][i] = to_float(from_float<T>(r[j][i] + d[i]));
+            if (vec && live == 8) {
+                store8(sum + at, r[j]);
+            } else {
+#pragma unroll
+                for (int i = 0; i < 8; ++i)
+                    if (i < live) sum[at + i] = from_float<T>(r[j][i]);
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const double d = r[j][i];
+            ss = fma(d, d, ss);
+        }
+    }
+#pragma unroll
+    for (int o = 16; o; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+    if ((threadIdx.x & 31) == 0) red[warp] = ss;
+    __syncthreads();
+    ss = 0.0;
+    for (int w = 0; w < static_cast<int>(blockDim.x >> 5); ++w) ss += red[w];
+    const double rs = 1.0 / sqrt(ss / k + kNormEps);
+    const int per_row = (k + kFp8Block - 1) / kFp8Block;
+#pragma unroll
+    for (int j = 0; j < CHUNKS; ++j) {
+        const int c = static_cast<int>(threadIdx.x + j * blockDim.x) * 8;
+        const int live = max(0, min(8, k - c));
+        float w[8];
+        load8_ragged(gamma + (live ? c : 0), live, vec, w);
+        unsigned long long a = 0;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) a = umax(a, abs_bits(static_cast<double>(r[j][i]) * static_cast<double>(w[i])));
+#pragma unroll
+        for (int o = kLanesPerGroup / 2; o; o >>= 1) a = umax(a, __shfl_xor_sync(0xffffffffu, a, o));
+        const double top = __longlong_as_double(static_cast<long long>(a)) * rs;
+        float s = static_cast<float>(top / static_cast<double>(kFp8Max));
+        if (!(s <= 3.4e38f)) s = __uint_as_float(0x7fffffffu);
+        GroupScale g = group_scale(s);
+        const float f = s > 0.0f ? static_cast<float>(rs / static_cast<double>(s)) : 0.0f;
+        g.exact_only |= !(f < 1e30f) || !(f > 1e-30f && fabs(top) < 1e30);
+        const uint2 b = quantise8(
+            g, [&](int i) { return r[j][i] * w[i] * f; },
+            [&](int i) { return static_cast<double>(r[j][i]) * static_cast<double>(w[i]) * rs; });
+        if (live) {
+            store_bytes(q + row * ldq + c, b, live);
+            if (threadIdx.x % kLanesPerGroup == 0) scale[row * per_row + c / kFp8Block] = s;
+        }
+    }
+}
+
+template <typename T>
+cudaError_t launch_norm_typed(const void* delta, const void* residual, void* sum, const float* gamma, uint8_t* q,
+                              size_t ldq, float* scale, int n, int k, cudaStream_t s) {
+    const bool vec = (static_cast<size_t>(k) * sizeof(T)) % 16 == 0;
+    const int chunks = (k + 7) / 8;
+    const T *d = static_cast<const T*>(delta), *r = static_cast<const T*>(residual);
+    T* o = static_cast<T*>(sum);
+    count_launch();
+    auto threads = [&](int per) { return ((chunks + per - 1) / per + 31) / 32 * 32; };
+    if (chunks <= 256) add_rmsnorm_fp8_kernel<T, 1><<<n, threads(1), 0, s>>>(d, r, o, gamma, q, ldq, scale, k, vec);
+    else if (chunks <= 1024) add_rmsnorm_fp8_kernel<T, 2><<<n, threads(2), 0, s>>>(d, r, o, gamma, q, ldq, scale, k, vec);
+    else add_rmsnorm_fp8_kernel<T, 4><<<n, threads(4), 0, s>>>(d, r, o, gamma, q, ldq, scale, k, vec);
+    return cudaGetLastError();
+}
+
+template <typename T>
+cudaError_t launch_quantize_typed(const void* xv, size_t ldx, uint8_t* q, size_t ldq, float* scale, int n, int k,
+                                  int rows, int num_sms, cudaStream_t s) {
+    const T* x = static_cast<const T*>(xv);
+    const bool vec = reinterpret_cast<uintptr_t>(x) % 16 == 0 && (ldx * sizeof(T)) % 16 == 0;
+    const uint32_t per_row = static_cast<uint32_t>((k - 1) / kFp8Block + 1);
+    count_launch();
+    if (rows == 1) {
+        const uint32_t groups = static_cast<uint32_t>(n) * per_row;
+        const uint32_t ctas = (groups + 15) / 16, most = static_cast<uint32_t>(num_sms) * 32;
+        quantize_rows_kernel<T><<<ctas < most ? ctas : most, 256, 0, s>>>(x, ldx, q, ldq, scale, groups,
+                                                                          FastDiv(per_row), k, vec);
+    } else {
+        const uint32_t blocks = static_cast<uint32_t>((n - 1) / kFp8Block + 1) * per_row;
+        quantize_blocks_kernel<T><<<blocks, 256, 0, s>>>(x, ldx, q, ldq, scale, FastDiv(per_row), n, k, vec);
+    }
+    return cudaGetLastError();
+}
+
+}  // namespace
+
+cudaError_t launch_quantize_fp8(int dtype, const void* x, size_t ldx, uint8_t* q, size_t ldq, float* scale, int n, int k,
+                                int rows, int num_sms, cudaStream_t s) {
+    switch (dtype) {
+        case kF32: return launch_quantize_typed<float>(x, ldx, q, ldq, scale, n, k, rows, num_sms, s);
+        case kBF16: return launch_quantize_typed<__nv_bfloat16>(x, ldx, q, ldq, scale, n, k, rows, num_sms, s);
+        case kF16: return launch_quantize_typed<__half>(x, ldx, q, ldq, scale, n, k, rows, num_sms, s);
+        default: return cudaErrorInvalidValue;
+    }
+}
+
+cudaError_t launch_add_rmsnorm_fp8(int dtype, const void* delta, const void* residual, void* sum, const float* gamma,
+                                   uint8_t* q, size_t ldq, float* scale, int n, int k, cudaStream_t s) {
+    switch (dtype) {
+        case kF32: return launch_norm_typed<float>(delta, residual, sum, gamma, q, ldq, scale, n, k, s);
+        case kBF16: return launch_norm_typed<__nv_bfloat16>(delta, residual, sum, gamma, q, ldq, scale, n, k, s);
+        case kF16: return launch_norm_typed<__half>(delta, residual, sum, gamma, q, ldq, scale, n, k, s);
+        default: return cudaErrorInvalidValue;
+    }
+}
+
+}  // namespace xl

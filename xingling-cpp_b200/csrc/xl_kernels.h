@@ -387,4 +387,26 @@ cudaError_t launch_add_rows(float* x, const float* d, int n, cudaStream_t s);
 cudaError_t launch_attn_prefill(const float* qkv, const float* kc, const float* vc, float* out, float* out_lo, int n,
                                 int heads, int max_ctx, cudaStream_t s, int p0 = 0);
 
+// ---- 8-bit projections and the paged cache (quant_fp8.cu, linear_fp8.cu, paged.cu) ----
+// Element types of the entry points that take one (XL_F32, XL_BF16, XL_F16).
+enum DType : int { kF32 = 0, kBF16 = 1, kF16 = 2 };
+constexpr int kFp8Block = 128;  // columns (and, for weights, rows) that share an e4m3 scale
+// q, scale of [n][k] rows: one scale per 128 columns of one row (rows = 1) or of 128 rows (rows = 128).
+cudaError_t launch_quantize_fp8(int dtype, const void* x, size_t ldx, uint8_t* q, size_t ldq, float* scale, int n, int k,
+                                int rows, int num_sms, cudaStream_t s);
+// sum = residual + delta (delta may be null: then sum is not written), q and scale of its RMSNorm.
+constexpr int kNormMaxK = 32768;  // a row is kept in one CTA's registers
+cudaError_t launch_add_rmsnorm_fp8(int dtype, const void* delta, const void* residual, void* sum, const float* gamma,
+                                   uint8_t* q, size_t ldq, float* scale, int n, int k, cudaStream_t s);
+// y (+)= xq . wq^T with the scales, mode as GemvMode (Plain / SwiGLU / Residual).
+cudaError_t launch_linear_fp8(int mode, int dtype, const uint8_t* xq, size_t ldx, const float* xs, const uint8_t* wq,
+                              size_t ldw, const float* ws, const float* bias, void* y, int n, int m, int k, int num_sms,
+                              cudaStream_t s);
+struct PagedCache;  // paged.h
+cudaError_t launch_kv_append_paged(const PagedCache& pc, int dtype, const void* qkv, const float* rope, int rope_len,
+                                   const int* row_seq, const int* row_pos, int rows, int heads, cudaStream_t s);
+size_t attn_paged_ws_bytes(int batch, int heads, int kv_heads);
+cudaError_t launch_attn_decode_paged(const PagedCache& pc, int dtype, const void* qkv, const float* rope, int rope_len,
+                                     const int* pos, void* out, int heads, void* ws, int num_sms, cudaStream_t s);
+
 }  // namespace xl
