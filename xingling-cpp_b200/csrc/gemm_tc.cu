@@ -26,6 +26,7 @@
 
 #include <algorithm>
 
+#include "tcgen05.cuh"
 #include "xl_device.cuh"
 #include "xl_kernels.h"
 
@@ -38,82 +39,9 @@ constexpr int kBN = 128;               // tokens per tile (MMA N; 256-token tile
 constexpr int kBK = 32;                // floats per K-block (128 B rows)
 constexpr int kTileBytes = kBM * kBK * 4;  // 16 KB: one 128-row operand tile of a K-block
 constexpr int kGemmThreads = 192;
-constexpr uint32_t kSpinLimit = 1u << 26;
-constexpr unsigned long long kWaitLimitNs = 200ull * 1000 * 1000;  // a tile's operands land in microseconds
 constexpr int kGemmPartial = 4;  // epilogue: raw slice accumulator into the split-K workspace
 constexpr int kGemmScores = 5;   // attention: S[z][n][m] = q_n . k_m per head z (tiles above the diagonal skipped)
 constexpr int kGemmPV = 6;       // attention: O[n][z*64 + f] (+ lo) = P[z][n][:] . V[:][f], keys up to the tile's last query
-
-__device__ __forceinline__ uint32_t smem_u32(const void* p) {
-    return static_cast<uint32_t>(__cvta_generic_to_shared(p));
-}
-__device__ __forceinline__ void mbar_init(uint64_t* bar, uint32_t count) {
-    asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(smem_u32(bar)), "r"(count) : "memory");
-}
-__device__ __forceinline__ void mbar_expect_tx(uint64_t* bar, uint32_t bytes) {
-    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(smem_u32(bar)), "r"(bytes)
-                 : "memory");
-}
-__device__ __forceinline__ bool mbar_try_wait(uint64_t* bar, uint32_t parity) {
-    uint32_t ok;
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
-        "selp.u32 %0, 1, 0, p;\n\t}"
-        : "=r"(ok)
-        : "r"(smem_u32(bar)), "r"(parity)
-        : "memory");
-    return ok != 0;
-}
-__device__ __forceinline__ unsigned long long globaltimer_ns() {
-    unsigned long long t;
-    asm volatile("mov.u64 %0, %globaltimer;" : "=l"(t));
-    return t;
-}
-// Bounded by polls and by wall-clock time (a try_wait may suspend the thread).
-__device__ bool wait_bar(uint64_t* bar, uint32_t parity, int* err) {
-    uint32_t it = 0;
-    unsigned long long t0 = 0;
-    while (!mbar_try_wait(bar, parity)) {
-        ++it;
-        if ((it & 63u) == 0) {
-            const unsigned long long now = globaltimer_ns();
-            if (t0 == 0) t0 = now;
-            if (it >= kSpinLimit || now - t0 > kWaitLimitNs) {
-                if (err) atomicOr(err, 4);
-                return false;
-            }
-        }
-    }
-    return true;
-}
-// 2D TMA tile load (no multicast): box {32 floats, 128 rows} at (x, y).
-__device__ __forceinline__ void tma_load_2d(void* dst, const CUtensorMap* map, int x, int y, uint64_t* bar) {
-    asm volatile(
-        "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::
-            "r"(smem_u32(dst)),
-        "l"(map), "r"(x), "r"(y), "r"(smem_u32(bar))
-        : "memory");
-}
-// A 2D tile of a tensor map into L2 only (no shared memory, no multicast).
-__device__ __forceinline__ void tma_prefetch_2d(const CUtensorMap* map, int x, int y) {
-    asm volatile("cp.async.bulk.prefetch.tensor.2d.L2.global.tile [%0, {%1, %2}];" ::"l"(map), "r"(x), "r"(y)
-                 : "memory");
-}
-// Shared-memory matrix descriptor: K-major, SWIZZLE_128B, 8-row groups 1024 B apart.
-__device__ __forceinline__ uint64_t umma_desc(uint32_t saddr) {
-    uint64_t d = 0;
-    d |= static_cast<uint64_t>((saddr & 0x3FFFFu) >> 4);   // start address
-    d |= static_cast<uint64_t>(1) << 16;                  // leading byte offset (unused for swizzled K-major)
-    d |= static_cast<uint64_t>(1024 >> 4) << 32;          // stride byte offset
-    d |= static_cast<uint64_t>(1) << 46;                  // descriptor version (sm_100)
-    d |= static_cast<uint64_t>(2) << 61;                  // SWIZZLE_128B
-    return d;
-}
-__device__ __forceinline__ void mma_commit(uint64_t* bar) {
-    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar))
-                 : "memory");
-}
 
 __device__ __forceinline__ void mma_tf32_i(uint32_t tmem_d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
     asm volatile(
@@ -403,6 +331,22 @@ cudaError_t make_tile_map(CUtensorMap* map, const float* base, int rows, int col
     const cuuint32_t box[2] = {kBK, static_cast<cuuint32_t>(box_rows)};
     const cuuint32_t elem[2] = {1, 1};
     const CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 2, const_cast<float*>(base), dims, strides, box, elem,
+                          CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                          CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    return r == CUDA_SUCCESS ? cudaSuccess : cudaErrorInvalidValue;
+}
+
+// Row-major [rows][cols] bytes with rows of `pitch` bytes as a 2D TMA map with {128, box_rows} boxes, 128B swizzle.
+cudaError_t make_byte_map(CUtensorMap* map, const uint8_t* base, int rows, int cols, size_t pitch, int box_rows) {
+    EncodeTiledFn fn = encode_fn();
+    if (!fn) return cudaErrorNotSupported;
+    if (reinterpret_cast<uintptr_t>(base) % 16 || pitch % 16 || box_rows <= 0 || box_rows > 256)
+        return cudaErrorInvalidValue;
+    const cuuint64_t dims[2] = {static_cast<cuuint64_t>(cols), static_cast<cuuint64_t>(rows)};
+    const cuuint64_t strides[1] = {static_cast<cuuint64_t>(pitch)};
+    const cuuint32_t box[2] = {128, static_cast<cuuint32_t>(box_rows)};
+    const cuuint32_t elem[2] = {1, 1};
+    const CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<uint8_t*>(base), dims, strides, box, elem,
                           CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
                           CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     return r == CUDA_SUCCESS ? cudaSuccess : cudaErrorInvalidValue;

@@ -324,6 +324,8 @@ struct TcOperands {
     bool wide = false;
 };
 cudaError_t make_tile_map(CUtensorMap* map, const float* base, int rows, int cols, int box_rows = 128);
+// An e4m3 matrix with rows of `pitch` bytes: {128, box_rows} boxes, 128B swizzle.
+cudaError_t make_byte_map(CUtensorMap* map, const uint8_t* base, int rows, int cols, size_t pitch, int box_rows);
 // C[N][M] (+)= X[N][K] . W[M][K]^T + b with the 3xTF32 split; SwiGLU writes C and C_lo as [N][M/2].
 // With a workspace (ws, ws_floats) and fewer output tiles than SMs, K is split
 // into slices whose partial sums are added in slice order by a second kernel.
