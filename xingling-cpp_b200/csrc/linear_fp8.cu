@@ -52,9 +52,12 @@ struct Tile {
     static constexpr int kTokens = CG * kRows;          // of the tile, all CTAs
     static constexpr int kFeatures = CG * 128;          // each CTA loads 128 of them
     static constexpr int kEpiWarps = 4 * CG;            // each drains 32 lanes x 128 columns
-    static constexpr int kThreads = 64 + 32 * kEpiWarps;
+    // two issuing warps (the pair's tiling: a warpgroup, so that registers can be moved to the epilogue's)
+    static constexpr int kEpiFirst = CG == 1 ? 2 : 4;
+    static constexpr int kThreads = 32 * (kEpiFirst + kEpiWarps);
     static constexpr int kAccs = 512 / kFeatures;       // TMEM accumulators
-    static constexpr int kStoreBytes = kEpiWarps * 32 * kStagePitch * 4;
+    static constexpr int kWarpStore = 32 * kStagePitch + 128;  // floats: a warp's staging rows and its bias
+    static constexpr int kStoreBytes = kEpiWarps * kWarpStore * 4;
     // kind::f8f6f4, e4m3 x e4m3, fp32 sums, K-major operands
     static constexpr uint32_t kIdesc = (1u << 4) | (static_cast<uint32_t>(kFeatures >> 3) << 17) |
                                        (static_cast<uint32_t>(kTokens >> 4) << 24);
@@ -83,6 +86,11 @@ __device__ __forceinline__ uint32_t cluster_addr(uint32_t saddr, uint32_t rank) 
 // Every thread of every CTA of a cluster comes here on every path, so it ends.
 __device__ __forceinline__ void cluster_sync() {
     asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+
+// A whole warp waits, and agrees on whether the wait ended in time.
+__device__ __forceinline__ bool wait_warp(uint64_t* bar, uint32_t parity) {
+    return __all_sync(0xffffffffu, mbar_try_wait(bar, parity) || wait_bar(bar, parity, nullptr));
 }
 
 template <int CG>
@@ -128,20 +136,29 @@ __device__ __forceinline__ void commit(uint64_t* bar) {
             : "memory");
 }
 
-// 16 columns of the warp's 32 TMEM lanes.
-__device__ __forceinline__ void tmem_load16(uint32_t addr, uint32_t (&r)[16]) {
+// 32 columns of the warp's 32 TMEM lanes.
+__device__ __forceinline__ void tmem_load32(uint32_t addr, uint32_t (&r)[32]) {
     asm volatile(
-        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, "
-        "[%16];"
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+        "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
         : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
-          "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+          "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
+          "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
+          "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
         : "r"(addr));
 }
 // The loads so far have landed; naming the registers keeps their uses behind the wait.
-__device__ __forceinline__ void tmem_wait16(uint32_t (&r)[16]) {
+__device__ __forceinline__ void tmem_wait64(uint32_t (&a)[32], uint32_t (&b)[32]) {
     asm volatile("tcgen05.wait::ld.sync.aligned;"
-                 : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]),
-                   "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15])
+                 : "+r"(a[0]), "+r"(a[1]), "+r"(a[2]), "+r"(a[3]), "+r"(a[4]), "+r"(a[5]), "+r"(a[6]), "+r"(a[7]),
+                   "+r"(a[8]), "+r"(a[9]), "+r"(a[10]), "+r"(a[11]), "+r"(a[12]), "+r"(a[13]), "+r"(a[14]),
+                   "+r"(a[15]), "+r"(a[16]), "+r"(a[17]), "+r"(a[18]), "+r"(a[19]), "+r"(a[20]), "+r"(a[21]),
+                   "+r"(a[22]), "+r"(a[23]), "+r"(a[24]), "+r"(a[25]), "+r"(a[26]), "+r"(a[27]), "+r"(a[28]),
+                   "+r"(a[29]), "+r"(a[30]), "+r"(a[31]), "+r"(b[0]), "+r"(b[1]), "+r"(b[2]), "+r"(b[3]), "+r"(b[4]),
+                   "+r"(b[5]), "+r"(b[6]), "+r"(b[7]), "+r"(b[8]), "+r"(b[9]), "+r"(b[10]), "+r"(b[11]), "+r"(b[12]),
+                   "+r"(b[13]), "+r"(b[14]), "+r"(b[15]), "+r"(b[16]), "+r"(b[17]), "+r"(b[18]), "+r"(b[19]),
+                   "+r"(b[20]), "+r"(b[21]), "+r"(b[22]), "+r"(b[23]), "+r"(b[24]), "+r"(b[25]), "+r"(b[26]),
+                   "+r"(b[27]), "+r"(b[28]), "+r"(b[29]), "+r"(b[30]), "+r"(b[31])
                  :
                  : "memory");
 }
@@ -159,6 +176,15 @@ __device__ __forceinline__ void fma2(unsigned long long& acc, unsigned long long
     asm("fma.rn.f32x2 %0, %1, %2, %0;" : "+l"(acc) : "l"(a), "l"(b));
 }
 
+// acc[first ..] += s * 32 columns
+__device__ __forceinline__ void scale_in(unsigned long long (&acc)[64], int first, const uint32_t (&r)[32],
+                                         unsigned long long s2) {
+#pragma unroll
+    for (int i = 0; i < 16; ++i) fma2(acc[first + i], pack2(r[2 * i], r[2 * i + 1]), s2);
+}
+
+__device__ __forceinline__ float silu_fast(float v) { return __fdividef(v, 1.0f + expf(-v)); }  // within 5 ulp
+
 template <typename T>
 __device__ __forceinline__ void put(T* dst, float v, int mode) {
     *dst = from_float<T>(mode == kGemvResidual ? to_float(*dst) + v : v);
@@ -166,51 +192,50 @@ __device__ __forceinline__ void put(T* dst, float v, int mode) {
 
 // 32 tokens x 128 features in registers (a token a lane) to y, 16 outputs a
 // row at a time through the warp's staging rows, so that stores are 16 bytes
-// a lane along the rows.
+// a lane along the rows.  bias: the warp's 128 values in shared memory.
 template <typename T>
 __device__ __forceinline__ void store_rows(const unsigned long long (&acc)[64], const LinearParams& p, int tok0, int j0,
-                                           float* st, int lane) {
-    const int wide = p.mode == kGemvSwiGLU ? p.m / 2 : p.m;
+                                           float* st, const float4* bias, int lane) {
+    const bool swiglu = p.mode == kGemvSwiGLU;
+    const int wide = swiglu ? p.m / 2 : p.m;
     const bool vec = (static_cast<size_t>(wide) * sizeof(T)) % 16 == 0;
+    const int rows = min(32, p.n - tok0);
     T* y = static_cast<T*>(p.y);
     constexpr int kPer = 16 / sizeof(T);  // outputs of a 16-byte store
+    float4* row = reinterpret_cast<float4*>(st + lane * kStagePitch);
 #pragma unroll
     for (int ch = 0; ch < 8; ++ch) {
-        int o0 = j0 + ch * 16;
-        if (p.mode == kGemvSwiGLU) {
-            if (ch >= 4) break;
-            o0 = j0 / 2 + ch * 16;
-        }
+        if (swiglu && ch >= 4) break;
+        const int o0 = (swiglu ? j0 / 2 : j0) + ch * 16;
         if (o0 >= wide) break;
-        float v[16];
-        if (p.mode == kGemvSwiGLU) {
+        if (swiglu) {
 #pragma unroll
-            for (int i = 0; i < 16; ++i) {
-                const float2 ac = unpack2(acc[((ch & 3) * 16 + i)]);
-                const int j = j0 + (ch & 3) * 32 + 2 * i;
-                const bool on = p.bias && j < p.m;
-                const float a = ac.x + (on ? p.bias[j] : 0.0f), c = ac.y + (on ? p.bias[j + 1] : 0.0f);
-                v[i] = silu(a) * c;
+            for (int i = 0; i < 4; ++i) {
+                float v[4];
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const float4 b = bias[(ch & 3) * 8 + 2 * i + h];
+                    const float2 e = unpack2(acc[(ch & 3) * 16 + 4 * i + 2 * h]), f = unpack2(acc[(ch & 3) * 16 + 4 * i + 2 * h + 1]);
+                    v[2 * h] = silu_fast(e.x + b.x) * (e.y + b.y);
+                    v[2 * h + 1] = silu_fast(f.x + b.z) * (f.y + b.w);
+                }
+                row[i] = make_float4(v[0], v[1], v[2], v[3]);
             }
         } else {
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const float2 a = unpack2(acc[ch * 8 + i]);
-                const int j = o0 + 2 * i;
-                v[2 * i] = a.x + (p.bias && j < p.m ? p.bias[j] : 0.0f);
-                v[2 * i + 1] = a.y + (p.bias && j + 1 < p.m ? p.bias[j + 1] : 0.0f);
+            for (int i = 0; i < 4; ++i) {
+                const float4 b = bias[ch * 4 + i];
+                const float2 e = unpack2(acc[ch * 8 + 2 * i]), f = unpack2(acc[ch * 8 + 2 * i + 1]);
+                row[i] = make_float4(e.x + b.x, e.y + b.y, f.x + b.z, f.y + b.w);
             }
         }
-        float4* row = reinterpret_cast<float4*>(st + lane * kStagePitch);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) row[i] = make_float4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
         __syncwarp();
         if (vec && o0 + 16 <= wide) {
             constexpr int kLanes = 16 / kPer;  // lanes a row
 #pragma unroll
             for (int r0 = 0; r0 < 32; r0 += 32 / kLanes) {
                 const int r = r0 + lane / kLanes, c = lane % kLanes * kPer;
-                if (tok0 + r < p.n) {
+                if (r < rows) {
                     const float* src = st + r * kStagePitch + c;
                     T* dst = y + static_cast<size_t>(tok0 + r) * wide + o0 + c;
                     uint4 out;
@@ -227,10 +252,10 @@ __device__ __forceinline__ void store_rows(const unsigned long long (&acc)[64], 
                 }
             }
         } else {
-#pragma unroll 1
-            for (int r0 = 0; r0 < 32; r0 += 2) {
+#pragma unroll 4
+            for (int r0 = 0; r0 < rows; r0 += 2) {
                 const int r = r0 + lane / 16, c = lane % 16;
-                if (tok0 + r < p.n && o0 + c < wide)
+                if (r < rows && o0 + c < wide)
                     put(y + static_cast<size_t>(tok0 + r) * wide + o0 + c, st[r * kStagePitch + c], p.mode);
             }
         }
@@ -252,7 +277,7 @@ __global__ void __launch_bounds__(Tile<CG>::kThreads, 1)
     uint64_t* freed = done + TL::kAccs;   // its columns have been read
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(freed + TL::kAccs);
 
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int warp = __shfl_sync(0xffffffffu, static_cast<int>(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
     const uint32_t rank = CG == 2 || p.split > 1 ? cluster_rank() : 0u;
     const int group = CG == 2 ? 2 : p.split;  // CTAs that share a tile
     const int unit = static_cast<int>(blockIdx.x) / group, units = static_cast<int>(gridDim.x) / group;
@@ -292,47 +317,52 @@ __global__ void __launch_bounds__(Tile<CG>::kThreads, 1)
     // Token tiles advance fastest: the CTAs that run together share W tiles
     // and, over the whole product, either operand stays in L2.
     const uint32_t a_bytes = static_cast<uint32_t>(p.x_rows) * kFp8Block;
+    // The pair's epilogue needs 128 sums and 64 columns in flight a thread: 384 threads launch with 168
+    // registers, the issuing warpgroup keeps 40, the others take 232 (128 x 40 + 256 x 232 = 384 x 168).
+    if (CG == 2 && warp < TL::kEpiFirst) asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
+    // Both issuing warps run their loops converged and elect one lane to issue.
     if (warp == 0) {
-        if (lane == 0) {
-            int s = 0;
-            uint32_t ph = 0, issued = 0;
-            bool ok = true;
-            for (int t = unit; t < tiles && ok; t += units) {
-                const int tn = t % p.tiles_n, tm = t / p.tiles_n;
-                const int y_x = tn * TL::kTokens + (CG == 2 ? static_cast<int>(rank) * kRows : 0);
-                const int y_w = tm * TL::kFeatures + (CG == 2 ? static_cast<int>(rank) * 128 : 0);
-                for (int kb = kb0; kb < kb1; ++kb) {
-                    if (!wait_bar(&empty[s], ph ^ 1u, nullptr)) {
-                        ok = false;
-                        break;
-                    }
-                    const uint32_t st = smem_u32(ring + s * p.stage_bytes);
-                    uint32_t bar = smem_u32(&full[s]);
-                    if (CG == 2) bar = cluster_addr(bar, 0);
+        int s = 0;
+        uint32_t ph = 0, issued = 0;
+        bool ok = true;
+        for (int t = unit; t < tiles && ok; t += units) {
+            const int tn = t % p.tiles_n, tm = t / p.tiles_n;
+            const int y_x = tn * TL::kTokens + (CG == 2 ? static_cast<int>(rank) * kRows : 0);
+            const int y_w = tm * TL::kFeatures + (CG == 2 ? static_cast<int>(rank) * 128 : 0);
+            for (int kb = kb0; kb < kb1; ++kb) {
+                if (!wait_warp(&empty[s], ph ^ 1u)) {
+                    ok = false;
+                    break;
+                }
+                const uint32_t st = smem_u32(ring + s * p.stage_bytes);
+                uint32_t bar = smem_u32(&full[s]);
+                if (CG == 2) bar = cluster_addr(bar, 0);
+                if (elect_one()) {
                     if (CG == 1 || rank == 0) mbar_expect_tx(&full[s], CG * (a_bytes + kOpBytes));
-                    load_tile<CG>(st, &map_x, kb * kFp8Block, y_x, bar);
                     load_tile<CG>(st + a_bytes, &map_w, kb * kFp8Block, y_w, bar);
-                    ++issued;
-                    if (++s == p.stages) s = 0, ph ^= 1u;
+                    load_tile<CG>(st, &map_x, kb * kFp8Block, y_x, bar);
                 }
+                __syncwarp();
+                ++issued;
+                if (++s == p.stages) s = 0, ph ^= 1u;
             }
-            if (!ok && (CG == 1 || rank == 0)) {
-                // the copies in flight land before the CTA leaves
-                for (uint32_t i = 0; i < min(issued, static_cast<uint32_t>(p.stages)); ++i) {
-                    if (s == 0) s = p.stages, ph ^= 1u;
-                    --s;
-                    wait_bar(&full[s], ph, nullptr);
-                }
+        }
+        if (!ok && (CG == 1 || rank == 0)) {
+            // the copies in flight land before the CTA leaves
+            for (uint32_t i = 0; i < min(issued, static_cast<uint32_t>(p.stages)); ++i) {
+                if (s == 0) s = p.stages, ph ^= 1u;
+                --s;
+                wait_warp(&full[s], ph);
             }
         }
     } else if (warp == 1) {
-        if (lane == 0 && (CG == 1 || rank == 0)) {
+        if (CG == 1 || rank == 0) {
             int s = 0, a = 0;
             uint32_t ph = 0, pa = 0;
             bool ok = true;
             for (int t = unit; t < tiles && ok; t += units) {
                 for (int kb = kb0; kb < kb1; ++kb) {
-                    if (!wait_bar(&freed[a], pa ^ 1u, nullptr) || !wait_bar(&full[s], ph, nullptr)) {
+                    if (!wait_warp(&freed[a], pa ^ 1u) || !wait_warp(&full[s], ph)) {
                         ok = false;
                         break;
                     }
@@ -340,23 +370,29 @@ __global__ void __launch_bounds__(Tile<CG>::kThreads, 1)
                     const uint32_t st = smem_u32(ring + s * p.stage_bytes);
                     const uint64_t da = umma_desc(st), db = umma_desc(st + a_bytes);
                     const uint32_t acc = tmem + static_cast<uint32_t>(a * TL::kFeatures);
+                    if (elect_one()) {
 #pragma unroll
-                    for (int ks = 0; ks < 4; ++ks)  // 32 columns = 32 bytes each
-                        mma_e4m3<CG>(acc, da + 2 * ks, db + 2 * ks, TL::kIdesc, ks != 0);
-                    commit<CG>(&empty[s]);
-                    commit<CG>(&done[a]);
+                        for (int ks = 0; ks < 4; ++ks)  // 32 columns = 32 bytes each
+                            mma_e4m3<CG>(acc, da + 2 * ks, db + 2 * ks, TL::kIdesc, ks != 0);
+                        commit<CG>(&empty[s]);
+                        commit<CG>(&done[a]);
+                    }
+                    __syncwarp();
                     if (++s == p.stages) s = 0, ph ^= 1u;
                     if (++a == TL::kAccs) a = 0, pa ^= 1u;
                 }
             }
         }
-    } else {
+    } else if (warp >= TL::kEpiFirst) {
+        if (CG == 2) asm volatile("setmaxnreg.inc.sync.aligned.u32 232;");
         // TMEM lanes are a warp's by its number modulo 4
-        const int q = warp & 3, half = (warp - 2) >> 2;
-        float* st = store + (warp - 2) * 32 * kStagePitch;
+        const int q = warp & 3, half = (warp - TL::kEpiFirst) >> 2;
+        float* st = store + (warp - TL::kEpiFirst) * TL::kWarpStore;
+        float* sb = st + 32 * kStagePitch;
         int a = 0;
         uint32_t pa = 0;
         bool ok = true;
+        const uint32_t freed0 = CG == 2 ? cluster_addr(smem_u32(freed), 0) : smem_u32(freed);
         for (int t = unit; t < tiles; t += units) {
             const int tn = t % p.tiles_n, tm = t / p.tiles_n;
             const int tok0 = tn * TL::kTokens + (CG == 2 ? static_cast<int>(rank) * kRows : 0) + 32 * q;
@@ -364,49 +400,64 @@ __global__ void __launch_bounds__(Tile<CG>::kThreads, 1)
             const bool work = tok0 < p.n && j0 < p.m;  // else the warp only keeps the accumulators moving
             const float* xs = p.xs + static_cast<size_t>(min(tok0 + lane, p.n - 1)) * p.blocks;
             const float* ws = p.ws + static_cast<size_t>(min(j0, p.m - 1) / kFp8Block) * p.blocks;
+            float bias[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int j = j0 + 32 * i + lane;
+                bias[i] = p.bias && j < p.m ? p.bias[j] : 0.0f;
+            }
             unsigned long long acc[64];
 #pragma unroll
             for (int i = 0; i < 64; ++i) acc[i] = 0;
-            float sx = kb0 < kb1 ? xs[kb0] : 0.0f, sw = kb0 < kb1 ? ws[kb0] : 0.0f;
+            float sx = xs[kb0], sw = ws[kb0];
+            bool ready = mbar_try_wait(&done[a], pa);
 #pragma unroll 1
             for (int kb = kb0; kb < kb1; ++kb) {
                 const float s = sx * sw;
-                if (kb + 1 < kb1) sx = xs[kb + 1], sw = ws[kb + 1];
-                if (ok) ok = __all_sync(0xffffffffu, wait_bar(&done[a], pa, nullptr));
+                const int next = min(kb + 1, kb1 - 1);
+                sx = xs[next], sw = ws[next];
+                if (ok && !__all_sync(0xffffffffu, ready)) ok = wait_warp(&done[a], pa);
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                if (work && ok) {
+                const bool drain = work && ok;
+                const unsigned long long s2 = pack2(__float_as_uint(s), __float_as_uint(s));
+                uint32_t r0[32], r1[32];
+                if (drain) {
                     const uint32_t ta = tmem + (static_cast<uint32_t>(32 * q) << 16) +
                                         static_cast<uint32_t>(a * TL::kFeatures + 128 * half);
-                    const unsigned long long s2 = pack2(__float_as_uint(s), __float_as_uint(s));
-                    uint32_t r0[16], r1[16];
-                    tmem_load16(ta, r0);
-#pragma unroll
-                    for (int c = 0; c < 8; c += 2) {
-                        tmem_wait16(r0);
-                        tmem_load16(ta + 16 * (c + 1), r1);
-#pragma unroll
-                        for (int i = 0; i < 8; ++i) fma2(acc[c * 8 + i], pack2(r0[2 * i], r0[2 * i + 1]), s2);
-                        tmem_wait16(r1);
-                        if (c + 2 < 8) tmem_load16(ta + 16 * (c + 2), r0);
-#pragma unroll
-                        for (int i = 0; i < 8; ++i) fma2(acc[(c + 1) * 8 + i], pack2(r1[2 * i], r1[2 * i + 1]), s2);
-                    }
+                    // two rounds of 64 columns in flight; the accumulator is handed back before the last sums
+                    tmem_load32(ta, r0);
+                    tmem_load32(ta + 32, r1);
+                    tmem_wait64(r0, r1);
+                    scale_in(acc, 0, r0, s2);
+                    tmem_load32(ta + 64, r0);
+                    scale_in(acc, 16, r1, s2);
+                    tmem_load32(ta + 96, r1);
+                    tmem_wait64(r0, r1);
                 }
                 asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
                 __syncwarp();
-                if (lane == 0) {
-                    uint32_t bar = smem_u32(&freed[a]);
-                    if (CG == 2) bar = cluster_addr(bar, 0);
-                    asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
-                }
+                if (elect_one())
+                    // only TMEM reads are ordered by this arrival (the fence above); a cluster-wide release of
+                    // memory would cost over 1000 clocks a K-block
+                    asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(freed0 + 8 * a) : "memory");
                 if (++a == TL::kAccs) a = 0, pa ^= 1u;
+                if (kb + 1 < kb1) ready = mbar_try_wait(&done[a], pa);  // asked early: the answer comes behind the sums
+                if (drain) {
+                    scale_in(acc, 32, r0, s2);
+                    scale_in(acc, 48, r1, s2);
+                }
             }
             if (!ok) {  // a wait ran out: the results say so
 #pragma unroll
                 for (int i = 0; i < 64; ++i) acc[i] = 0x7fffffff7fffffffull;
             }
             if (CG == 2 || p.split == 1) {
-                if (work) store_rows<T>(acc, p, tok0, j0, st, lane);
+                if (work) {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) sb[32 * i + lane] = bias[i];
+                    __syncwarp();
+                    store_rows<T>(acc, p, tok0, j0, st, reinterpret_cast<const float4*>(sb), lane);
+                }
             } else {
                 // every K-block of this CTA has been multiplied: the ring is free for the partial tile
                 float* part = reinterpret_cast<float*>(ring);
@@ -444,7 +495,7 @@ __global__ void __launch_bounds__(Tile<CG>::kThreads, 1)
                 }
                 if (p.bias) v[i] += p.bias[j + i];
             }
-            put(y + static_cast<size_t>(tn * kRows + r) * wide + j / step, step == 2 ? silu(v[0]) * v[1] : v[0], p.mode);
+            put(y + static_cast<size_t>(tn * kRows + r) * wide + j / step, step == 2 ? silu_fast(v[0]) * v[1] : v[0], p.mode);
         }
     }
     __syncwarp();
@@ -463,6 +514,15 @@ template <int CG, typename T>
 cudaError_t launch_tiled(const CUtensorMap& mx, const CUtensorMap& mw, const LinearParams& p, int grid, cudaStream_t s) {
     using TL = Tile<CG>;
     const int smem = p.stages * p.stage_bytes + TL::kStoreBytes + kBarBytes + 1024;
+    if (CG == 2) {
+        // the warpgroups' register shares have to fit what the CTA launches with, or the larger one never comes
+        static const bool fits = [] {
+            cudaFuncAttributes a{};
+            return cudaFuncGetAttributes(&a, linear_fp8_kernel<CG, T>) == cudaSuccess &&
+                   a.numRegs * TL::kThreads >= 128 * 40 + 256 * 232;
+        }();
+        if (!fits) return cudaErrorInvalidConfiguration;
+    }
     cudaError_t e = cudaFuncSetAttribute(linear_fp8_kernel<CG, T>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemLimit);
     if (e != cudaSuccess) return e;
     cudaLaunchConfig_t cfg{};
@@ -481,6 +541,150 @@ cudaError_t launch_tiled(const CUtensorMap& mx, const CUtensorMap& mw, const Lin
     return cudaLaunchKernelEx(&cfg, linear_fp8_kernel<CG, T>, mx, mw, p);
 }
 
+// ---- few tokens: the weights stream through registers ----
+
+// 16 bytes of a row from column c on, zeros past k (the bytes between k and the row's pitch are not touched).
+__device__ __forceinline__ uint4 load_row16(const uint8_t* row, int c, int k) {
+    if (c + 16 <= k) return *reinterpret_cast<const uint4*>(row + c);
+    uint32_t w[4] = {0u, 0u, 0u, 0u};
+    for (int i = 0; i < 16; ++i)
+        if (c + i < k) w[i >> 2] |= static_cast<uint32_t>(row[c + i]) << (8 * (i & 3));
+    return make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+__device__ __forceinline__ void mma_16x8x32(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
+                                            uint32_t b0, uint32_t b1) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k32.row.col.f32.e4m3.e4m3.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, "
+        "%3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+// One K-block's operands of a lane: weight rows g and g + 8, NT token tiles, 2
+// x 16 bytes each.  A lane reads 16 consecutive bytes where the MMA's layout
+// wants 4 x 4: the columns are permuted alike in both operands, so the sums
+// are the same.
+template <int NT>
+struct StreamBlock {
+    uint4 a[2][2], b[NT][2];
+    float s[NT][2];
+};
+
+struct StreamParams {
+    const uint8_t *xq, *wq;
+    size_t ldx, ldw;
+    const float *xs, *ws, *bias;
+    void* y;
+    int mode, n, m, k, blocks;
+};
+
+// 16 weight rows a CTA, its warps share the K-blocks and add up through shared
+// memory.  No TMEM, no barriers but one: a decode step's product is a stream
+// of weights, and every load of a CTA is in flight at once.
+template <int NT, int DEPTH, typename T>
+__global__ void __launch_bounds__(512) linear_fp8_stream_kernel(const StreamParams p) {
+    extern __shared__ float part[];  // [warps][16][NT * 8 + 1]
+    constexpr int kPitch = NT * 8 + 1;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = static_cast<int>(blockDim.x >> 5);
+    const int g = lane >> 2, t = lane & 3, row0 = static_cast<int>(blockIdx.x) * 16;
+    const uint8_t* wr[2];
+    const uint8_t* xr[NT];
+    const float* sx[NT][2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) wr[i] = p.wq + static_cast<size_t>(min(row0 + g + 8 * i, p.m - 1)) * p.ldw;
+#pragma unroll
+    for (int i = 0; i < NT; ++i) {
+        xr[i] = p.xq + static_cast<size_t>(min(8 * i + g, p.n - 1)) * p.ldx;
+#pragma unroll
+        for (int j = 0; j < 2; ++j) sx[i][j] = p.xs + static_cast<size_t>(min(8 * i + 2 * t + j, p.n - 1)) * p.blocks;
+    }
+    const float* sw = p.ws + static_cast<size_t>(row0 / kFp8Block) * p.blocks;
+    auto load = [&](StreamBlock<NT>& o, int kb) {
+        if (kb >= p.blocks) return;
+        const int c = kb * kFp8Block + 16 * t;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+#pragma unroll
+            for (int i = 0; i < 2; ++i) o.a[i][h] = load_row16(wr[i], c + 64 * h, p.k);
+#pragma unroll
+            for (int i = 0; i < NT; ++i) o.b[i][h] = load_row16(xr[i], c + 64 * h, p.k);
+        }
+        const float w = sw[kb];
+#pragma unroll
+        for (int i = 0; i < NT; ++i)
+#pragma unroll
+            for (int j = 0; j < 2; ++j) o.s[i][j] = sx[i][j][kb] * w;
+    };
+    float acc[NT][4];
+#pragma unroll
+    for (int i = 0; i < NT; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) acc[i][j] = 0.0f;
+    StreamBlock<NT> ring[DEPTH];
+#pragma unroll
+    for (int d = 0; d < DEPTH; ++d) load(ring[d], warp + d * warps);
+    for (int kb = warp; kb < p.blocks; kb += DEPTH * warps) {
+#pragma unroll
+        for (int d = 0; d < DEPTH; ++d) {
+            const int at = kb + d * warps;
+            if (at < p.blocks) {
+                const StreamBlock<NT>& o = ring[d];
+#pragma unroll
+                for (int i = 0; i < NT; ++i) {
+                    float c[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        mma_16x8x32(c, o.a[0][h].x, o.a[1][h].x, o.a[0][h].y, o.a[1][h].y, o.b[i][h].x, o.b[i][h].y);
+                        mma_16x8x32(c, o.a[0][h].z, o.a[1][h].z, o.a[0][h].w, o.a[1][h].w, o.b[i][h].z, o.b[i][h].w);
+                    }
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) acc[i][j] = fmaf(c[j], o.s[i][j & 1], acc[i][j]);
+                }
+                load(ring[d], at + DEPTH * warps);
+            }
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < NT; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            part[(warp * 16 + g + (j >> 1) * 8) * kPitch + 8 * i + 2 * t + (j & 1)] = acc[i][j];
+    __syncthreads();
+    const int step = p.mode == kGemvSwiGLU ? 2 : 1, outs = 16 / step, wide = p.m / step;
+    T* y = static_cast<T*>(p.y);
+    for (int e = threadIdx.x; e < outs * p.n; e += blockDim.x) {
+        const int tok = e / outs, r = (e - tok * outs) * step, j = row0 + r;
+        if (j >= p.m) continue;
+        float v[2] = {0.0f, 0.0f};
+        for (int i = 0; i < step; ++i) {
+            for (int w = 0; w < warps; ++w) v[i] += part[(w * 16 + r + i) * kPitch + tok];
+            if (p.bias) v[i] += p.bias[j + i];
+        }
+        put(y + static_cast<size_t>(tok) * wide + j / step, step == 2 ? silu_fast(v[0]) * v[1] : v[0], p.mode);
+    }
+}
+
+template <int NT, int DEPTH, typename T>
+cudaError_t launch_stream_tiles(const StreamParams& p, int warps, cudaStream_t s) {
+    count_launch();
+    linear_fp8_stream_kernel<NT, DEPTH, T>
+        <<<(p.m - 1) / 16 + 1, 32 * warps, static_cast<size_t>(warps) * 16 * (NT * 8 + 1) * 4, s>>>(p);
+    return cudaGetLastError();
+}
+
+template <typename T>
+cudaError_t launch_stream(const StreamParams& p, int num_sms, cudaStream_t s) {
+    // enough warps to cover a memory round trip with the CTAs an SM holds; more where the rows are few
+    int warps = 4;
+    while (warps < 16 && 2 * warps <= p.blocks && static_cast<long long>(p.m / 16) * warps < 16ll * num_sms) warps *= 2;
+    if (p.n <= 8) return launch_stream_tiles<1, 4, T>(p, warps, s);
+    if (p.n <= 16) return launch_stream_tiles<2, 3, T>(p, warps, s);
+    return launch_stream_tiles<4, 2, T>(p, warps, s);
+}
+
+constexpr int kStreamTokens = 32;  // most tokens of the streaming kernel
+
 int cdiv(long long a, long long b) { return static_cast<int>((a + b - 1) / b); }
 
 }  // namespace
@@ -488,6 +692,15 @@ int cdiv(long long a, long long b) { return static_cast<int>((a + b - 1) / b); }
 cudaError_t launch_linear_fp8(int mode, int dtype, const uint8_t* xq, size_t ldx, const float* xs, const uint8_t* wq,
                               size_t ldw, const float* ws, const float* bias, void* y, int n, int m, int k, int num_sms,
                               cudaStream_t s) {
+    if (n <= kStreamTokens) {
+        const StreamParams p{xq, wq, ldx, ldw, xs, ws, bias, y, mode, n, m, k, cdiv(k, kFp8Block)};
+        switch (dtype) {
+            case kF32: return launch_stream<float>(p, num_sms, s);
+            case kBF16: return launch_stream<__nv_bfloat16>(p, num_sms, s);
+            case kF16: return launch_stream<__half>(p, num_sms, s);
+            default: return cudaErrorInvalidValue;
+        }
+    }
     LinearParams p{};
     p.xs = xs, p.ws = ws, p.bias = bias, p.y = y;
     p.mode = mode, p.n = n, p.m = m, p.blocks = cdiv(k, kFp8Block);

@@ -52,6 +52,18 @@ __device__ inline bool wait_bar(uint64_t* bar, uint32_t parity, int* err) {
     }
     return true;
 }
+// One lane of a converged warp.  The compiler knows that a branch on it holds
+// one thread, so the uniform operands of TMA and tcgen05 instructions inside
+// need no loop over the lanes (which `lane == 0` costs about 80 clocks each).
+__device__ __forceinline__ bool elect_one() {
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "elect.sync _|p, 0xffffffff;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok));
+    return ok != 0;
+}
 // 2D TMA tile load (no multicast): the map's box at (x, y).
 __device__ __forceinline__ void tma_load_2d(void* dst, const CUtensorMap* map, int x, int y, uint64_t* bar) {
     asm volatile(
