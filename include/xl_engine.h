@@ -401,7 +401,8 @@ XL_API int xl_op_linear_fp8(int mode, int dtype, const uint8_t* xq, size_t ldx, 
 
 /* A paged cache: pools k and v [num_pages][kv_heads][page_size][head_dim] of
  * dtype; page_table [batch][max_pages] (device ints) names the pages of each
- * sequence in order.  head_dim 64 or 128; max_pages * page_size <= 2^31 - 1.
+ * sequence in order.  head_dim 64 or 128; max_pages * page_size <= 2^31 - 1,
+ * num_pages * kv_heads * page_size <= 2^32 - 2, batch * heads < 2^30.
  * Entries past the pages that a sequence's positions need are not read.
  * Sequences may share pages that are not written any more.  The struct itself
  * is host memory, read during the call only. */

@@ -65,7 +65,7 @@ CACHE_FAULTS = [
     (dict(batch=0), "positive"), (dict(kv_heads=0), "positive"), (dict(page_size=0), "positive"),
     (dict(max_pages=0), "positive"), (dict(num_pages=-2), "positive"), (dict(head_dim=96), "head_dim"),
     (dict(kv_heads=3), "multiple"), (dict(page_size=1 << 16, max_pages=1 << 16), "2^31"),
-    (dict(batch=1 << 30), "2^30"), (dict(k=P + 8), "aligned"),
+    (dict(batch=1 << 30), "2^30"), (dict(k=P + 8), "aligned"), (dict(num_pages=1 << 30), "2^32"),
 ]
 
 

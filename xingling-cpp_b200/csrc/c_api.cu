@@ -501,6 +501,8 @@ const char* paged_fault(const xl_paged_kv* c, int heads) {
     if (c->head_dim != 64 && c->head_dim != 128) return "head_dim must be 64 or 128";
     if (heads % c->kv_heads) return "heads must be a multiple of kv_heads";
     if (static_cast<long long>(c->max_pages) * c->page_size > 0x7fffffffll) return "max_pages * page_size is over 2^31 - 1";
+    if (static_cast<double>(c->num_pages) * c->kv_heads * c->page_size > 4294967294.0)
+        return "num_pages * kv_heads * page_size is over 2^32 - 2";
     if (static_cast<long long>(c->batch) * heads > 0x3fffffffll) return "batch * heads is over 2^30 - 1";
     if (!aligned(c->k, 16) || !aligned(c->v, 16) || !aligned(c->page_table, 4)) return "cache pointers must be 16-byte aligned";
     return nullptr;
