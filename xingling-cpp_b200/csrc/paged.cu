@@ -61,33 +61,39 @@ __global__ void __launch_bounds__(256) kv_append_paged_kernel(const PagedCache p
 // One pass over the cache with the running maximum and sum of a softmax.  What
 // bounds it is reading the cache, so the work is cut by cache bytes: every
 // (sequence, key/value head, block of 8 or 16 query heads) is a "pair" of
-// chunks of 4 x kTile positions, the chunks of all pairs stand in one row, and
+// chunks of 64 positions, the chunks of all pairs stand in one row, and
 // every CTA takes an equal stretch of that row (lengths live on the device; a
 // CTA finds its stretch from them).  A pair that one CTA covers is finished
 // there; else its CTAs leave (maximum, sum, output) partials in the workspace
 // and the last to arrive (a ticket, nobody waits) merges them in CTA order, so
 // results do not depend on timing.
 //
-// Within a CTA each warp takes tiles of kTile positions with its own running
-// softmax.  Query heads that share a key/value head are the rows of
-// mma.sync tiles, so a byte of cache is read once for all of them and turned
-// into scores without shuffles.  The cache goes from global memory straight
-// into the MMA's register layout, 16 bytes a load: the columns that a lane
-// holds are a permutation of the MMA's, applied alike to both operands of the
-// scores (any order of d sums the same) and, for the values, undone when the
-// output is stored.
+// Within a CTA each warp takes tiles of 16 positions with its own running
+// softmax.  mma.sync does the sums: positions (for the output: columns of the
+// values) are its 16 rows, 8 query heads that share the key/value head its
+// columns, so a byte of cache is read once for all of them.  The cache goes
+// from global memory straight into the MMA's register layout, 16 bytes a
+// load: the columns that a lane holds are a permutation of the MMA's, applied
+// alike to both operands of the scores (any order of d sums the same) and,
+// for the values, undone when the output is stored.  The queries stand in
+// shared memory in that layout; the weights change from one MMA's result to
+// the next one's operand by an 8 x 8 transpose in registers (movmatrix).
 //
-// Precision: queries are split in two 16-bit halves (scaled by a power of two
-// so that they fit fp16), and so are the weights, which leaves 2^-17 of error
+// Precision: queries are split in two 16-bit halves (for fp16 scaled by a power
+// of two first), and so are the weights, which leaves 2^-17 of error
 // where rounding them would leave 2^-9; an fp32 cache runs as three TF32
 // products of split operands.  Sums, maxima and the running output are fp32.
 
 constexpr int kAttnWarps = 4;
-constexpr int kAttnMaxCtas = 592;            // 148 SMs x 4
+constexpr int kAttnMaxCtas = 740;            // 148 SMs x 5
+constexpr int kAttnShort = 8;                // chunks a CTA up to which stretches keep to one pair
+constexpr int kAttnTries = 6;
+constexpr int kMergeAhead = 8;
 constexpr int kAttnRows = 16;                // most query heads of a pair
 constexpr size_t kAttnSlotFloats = kAttnRows * (128 + 2);
 constexpr size_t kAttnPartBytes = kAttnMaxCtas * 2 * kAttnSlotFloats * 4;  // two partials a CTA
-constexpr uint32_t kNoRow = 0xffffffffu;     // masked or unreadable: zeros
+constexpr int kTile = 16;                    // positions of a warp's tile
+constexpr int kChunk = kAttnWarps * kTile;
 constexpr float kLog2e = 1.4426950408889634f;
 
 struct AttnParams {
@@ -113,6 +119,49 @@ __device__ __forceinline__ void store_io(void* p, int64_t i, float v, int io) {
     if (io == kF32) static_cast<float*>(p)[i] = v;
     else if (io == kBF16) static_cast<__nv_bfloat16*>(p)[i] = from_float<__nv_bfloat16>(v);
     else static_cast<__half*>(p)[i] = from_float<__half>(v);
+}
+
+template <int N, typename T>
+__device__ __forceinline__ void load_n(const T* p, float (&v)[N]) {
+    static_assert(N == 2 || N == 4, "2 or 4 elements, aligned to as many");
+    if constexpr (sizeof(T) == 4 && N == 4) {
+        const float4 x = *reinterpret_cast<const float4*>(p);
+        v[0] = x.x, v[1] = x.y, v[2] = x.z, v[3] = x.w;
+    } else if constexpr (sizeof(T) == 4 || N == 4) {
+        const uint2 x = *reinterpret_cast<const uint2*>(p);
+        const T* e = reinterpret_cast<const T*>(&x);
+#pragma unroll
+        for (int i = 0; i < N; ++i) v[i] = to_float(e[i]);
+    } else {
+        const uint32_t x = *reinterpret_cast<const uint32_t*>(p);
+        const T* e = reinterpret_cast<const T*>(&x);
+#pragma unroll
+        for (int i = 0; i < N; ++i) v[i] = to_float(e[i]);
+    }
+}
+template <int N>
+__device__ __forceinline__ void load_io_n(const void* p, int64_t i, int io, float (&v)[N]) {
+    if (io == kF32) load_n<N>(static_cast<const float*>(p) + i, v);
+    else if (io == kBF16) load_n<N>(static_cast<const __nv_bfloat16*>(p) + i, v);
+    else load_n<N>(static_cast<const __half*>(p) + i, v);
+}
+// 16 bytes of shared memory, read where it stands (kept in registers across the tiles they would spill).
+__device__ __forceinline__ uint4 load_shared(const uint4* p) {
+    uint4 v;
+    asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+                 : "r"(static_cast<uint32_t>(__cvta_generic_to_shared(p))));
+    return v;
+}
+
+// fp16 holds 5 exponent bits: a query row is scaled by a power of two so that its largest value is in [1, 2).
+template <typename C>
+constexpr bool kScaled = false;
+template <>
+constexpr bool kScaled<__half> = true;
+__device__ __forceinline__ int row_exponent(uint32_t bits) {
+    const int e = static_cast<int>(bits >> 23) - 127;
+    return bits == 0u || bits >= 0x7f800000u ? 0 : max(-120, min(120, e));
 }
 
 __device__ __forceinline__ uint32_t pack16(float lo, float hi, __nv_bfloat16) {
@@ -155,48 +204,47 @@ __device__ __forceinline__ void mma_tf32(float (&d)[4], const uint32_t (&a)[4], 
         : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-// Two products of a split value with an unsplit one (16-bit caches).
-template <typename C>
-__device__ __forceinline__ void mma_split(float (&d)[4], const uint32_t (&hi)[4], const uint32_t (&lo)[4], uint32_t b0,
-                                          uint32_t b1) {
-    mma16(d, hi, b0, b1, C{});
-    mma16(d, lo, b0, b1, C{});
+// An 8 x 8 matrix of 16-bit values, lane l holding row l / 4, columns 2 (l % 4) and the next: its transpose, held alike.
+__device__ __forceinline__ uint32_t transpose8(uint32_t v) {
+    uint32_t r;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+    return r;
 }
-// Three TF32 products: fp32 accuracy up to the dropped lo . lo (2^-22).  The
-// MMA reads the upper 19 bits of its operands, so a value is its own hi.
-__device__ __forceinline__ void mma_split3(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-    const uint32_t lo[4] = {tf32_lo(a[0]), tf32_lo(a[1]), tf32_lo(a[2]), tf32_lo(a[3])};
-    mma_tf32(d, a, b0, b1);
-    mma_tf32(d, a, tf32_lo(b0), tf32_lo(b1));
-    mma_tf32(d, lo, b0, b1);
+__device__ __forceinline__ float exp2_fast(float v) {  // 2^-22 relative, 0 below 2^-126
+    float r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
+    return r;
 }
 
 __device__ __forceinline__ uint32_t word(const uint4& v, int i) { return i == 0 ? v.x : i == 1 ? v.y : i == 2 ? v.z : v.w; }
 
-// C: cache type, D: head dim, WIDE: 16 query heads a pair (else 8, and the MMA's rows 8 .. 15 idle).
+// C: cache type, D: head dim, WIDE: 16 query heads a pair (else 8), as two column halves of the MMAs.
 template <typename C, int D, bool WIDE>
 struct AttnShape {
     static constexpr bool k32 = sizeof(C) == 4;
     static constexpr int kVec = 16 / sizeof(C);             // elements of a 16-byte load
-    static constexpr int kNT = k32 && D == 128 ? 1 : 2;     // 8-position MMA tiles of a warp tile
-    static constexpr int kTile = 8 * kNT;
-    static constexpr int kChunk = kAttnWarps * kTile;
     static constexpr int kKch = D / (4 * kVec);             // 16-byte loads of a lane per key row
     static constexpr int kVch = D / (8 * kVec);             // ... per value row
     static constexpr int kSteps = 2 * kKch;                 // MMA steps of a score
-    static constexpr int kRows = WIDE ? 16 : 8;
-    static constexpr int kQPitch = D + 4;
-    static constexpr int kSmemFloats = kRows * kQPitch + kAttnWarps * kRows * (D + 2);
-    static constexpr int kCtas = WIDE ? 2 : 3;              // an SM holds, by registers
+    static constexpr int kHalves = WIDE ? 2 : 1;
+    static constexpr int kRows = 8 * kHalves;
+    static constexpr int kPer = kVec / 2;                   // columns of a lane in a step
+    static constexpr int kFragFloats = kSteps * kHalves * 128;
+    static constexpr int kPartFloats = kAttnWarps * kRows * (D + 2);
+    static constexpr int kSmemFloats = kFragFloats > kPartFloats ? kFragFloats : kPartFloats;
+    // CTAs an SM holds, by registers: a lane keeps a tile's keys and values and its part of the output
+    // (4 and 5, with spills: 212 and 306 us where 3 takes 194, 64 sequences up to 8192 in bf16)
+    static constexpr int kCtas = D == 128 && (k32 || WIDE) ? 2 : 3;
 };
 
 template <typename C, int D, bool WIDE>
 __global__ void __launch_bounds__(128, (AttnShape<C, D, WIDE>::kCtas)) attn_decode_paged_kernel(const AttnParams p) {
     using S = AttnShape<C, D, WIDE>;
     extern __shared__ __align__(16) float smem[];
-    float* qs = smem;                              // [rows][D + 4] rotated queries
-    float* warp_part = smem + S::kRows * S::kQPitch;  // [warps][rows][D + 2]
+    uint4* frag = reinterpret_cast<uint4*>(smem);  // [steps][halves][32]: the queries in the MMA's layout, hi and lo
+    float* warp_part = smem;                       // [warps][rows][D + 2], once the queries are no longer read
     __shared__ int flag;
+    __shared__ uint32_t row_max[16];
     const PagedCache& pc = p.pc;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
     const int pairs = pc.kv_heads * p.blocks;  // of a sequence
@@ -205,25 +253,44 @@ __global__ void __launch_bounds__(128, (AttnShape<C, D, WIDE>::kCtas)) attn_deco
     const int limit = p.rope ? p.rope_len : 0;
 
     auto chunks_of = [&](int pos) {
-        return paged_pos_ok(pos, pc.max_pages, pc.page_size, limit) ? pos / S::kChunk + 1 : 1;
+        return paged_pos_ok(pos, pc.max_pages, pc.page_size, limit) ? pos / kChunk + 1 : 1;
     };
-    // Every warp adds up all sequences' chunks, then finds the sequence its CTA's stretch begins in.
-    long long total = 0;
-    for (int b0 = 0; b0 < pc.batch; b0 += 32) {
-        long long c = b0 + lane < pc.batch ? chunks_of(p.pos[b0 + lane]) : 0;
+    // The stretches are counted in units of `step` chunks of a pair.  Every warp adds up all sequences' units and
+    // finds the sequence that its CTA's stretch begins in; the positions are read once where a warp holds them all.
+    const int held = lane < pc.batch ? chunks_of(p.pos[lane]) : 0;
+    auto chunks_at = [&](int i) { return i < 32 ? held : i < pc.batch ? chunks_of(p.pos[i]) : 0; };
+    auto units_in_all = [&](int step) {
+        long long total = 0;
+        for (int b0 = 0; b0 < pc.batch; b0 += 32) {
+            long long c = (chunks_at(b0 + lane) + step - 1) / step;
 #pragma unroll
-        for (int o = 16; o; o >>= 1) c += __shfl_xor_sync(0xffffffffu, c, o);
-        total += c;
+            for (int o = 16; o; o >>= 1) c += __shfl_xor_sync(0xffffffffu, c, o);
+            total += c;
+        }
+        return total * pairs;
+    };
+    // Short work: the step is raised until every CTA has one unit at most, so that none takes parts of two pairs one
+    // after the other.  Long work, and more pairs than CTAs: single chunks, which cuts evenly.
+    int step = 1;
+    long long all = units_in_all(1);
+    if (all > gridDim.x && all <= static_cast<long long>(gridDim.x) * kAttnShort) {
+        int least = static_cast<int>((all + gridDim.x - 1) / gridDim.x);
+        for (int tries = 0; tries < kAttnTries; ++tries, ++least) {
+            const long long units = units_in_all(least);
+            if (units <= gridDim.x) {
+                step = least, all = units;
+                break;
+            }
+        }
     }
-    const long long all = total * pairs;
-    const long long grid = min(static_cast<long long>(gridDim.x), all);  // a chunk at least for every CTA that works
+    const long long grid = min(static_cast<long long>(gridDim.x), all);  // a unit at least for every CTA that works
     if (blockIdx.x >= grid) return;
     long long at = blockIdx.x * all / grid;
     const long long end = (blockIdx.x + 1) * all / grid;
     int b = 0;
-    long long first = 0;  // the row's index of sequence b's first chunk
+    long long first = 0;  // the row's index of sequence b's first unit
     for (int b0 = 0; b0 < pc.batch; b0 += 32) {
-        const long long own = b0 + lane < pc.batch ? chunks_of(p.pos[b0 + lane]) * static_cast<long long>(pairs) : 0;
+        const long long own = static_cast<long long>((chunks_at(b0 + lane) + step - 1) / step) * pairs;
         long long upto = own;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
@@ -242,20 +309,21 @@ __global__ void __launch_bounds__(128, (AttnShape<C, D, WIDE>::kCtas)) attn_deco
 
     while (at < end) {
         const int pos = p.pos[b];
-        const int nch = chunks_of(pos);
-        const int pair = static_cast<int>((at - first) / nch);
-        const int c0 = static_cast<int>((at - first) - static_cast<long long>(pair) * nch);
-        const int c1 = static_cast<int>(min(static_cast<long long>(nch), c0 + (end - at)));
+        const int nch = chunks_of(pos), nu = (nch + step - 1) / step;
+        const int pair = static_cast<int>((at - first) / nu);
+        const int u0 = static_cast<int>((at - first) - static_cast<long long>(pair) * nu);
+        const int u1 = static_cast<int>(min(static_cast<long long>(nu), u0 + (end - at)));
+        const int c0 = u0 * step, c1 = min(nch, u1 * step);
         const int kh = pair / p.blocks, blk = pair - kh * p.blocks;
         const int h0 = kh * p.group + blk * S::kRows, nh = min(S::kRows, p.group - blk * S::kRows);
         const int64_t out0 = (static_cast<int64_t>(b) * p.heads + h0) * D;
-        const long long pair_first = first + static_cast<long long>(pair) * nch;
-        at += c1 - c0;
-        if (pair == pairs - 1 && c1 == nch) {
-            first += static_cast<long long>(pairs) * nch;
+        const long long pair_first = first + static_cast<long long>(pair) * nu;
+        const int seq = b;
+        at += u1 - u0;
+        if (pair == pairs - 1 && u1 == nu) {
+            first += static_cast<long long>(pairs) * nu;
             ++b;
         }
-        const int seq = pair == pairs - 1 && c1 == nch ? b - 1 : b;
         if (!paged_pos_ok(pos, pc.max_pages, pc.page_size, limit)) {
             const float v = pos == -1 ? 0.0f : __int_as_float(0x7fffffff);
             for (int i = threadIdx.x; i < nh * D; i += 128) store_io(p.out, out0 + i, v, p.io);
@@ -264,25 +332,114 @@ __global__ void __launch_bounds__(128, (AttnShape<C, D, WIDE>::kCtas)) attn_deco
         const int* table = pc.page_table + static_cast<int64_t>(seq) * pc.max_pages;
         const int64_t qrow = seq * width;
 
-        // The rotated queries, and in the CTA that holds the last position its new key and value.
         __syncthreads();  // the last pair's shared memory has been read
-        for (int i = threadIdx.x; i < S::kRows * (D / 2); i += 128) {
-            const int r = i / (D / 2), j = i - r * (D / 2);
-            float a = 0.0f, c = 0.0f;
-            if (r < nh) {
-                const int64_t src = qrow + static_cast<int64_t>(h0 + r) * D + j;
-                a = load_io(p.qkv, src, p.io), c = load_io(p.qkv, src + D / 2, p.io);
-                if (p.rope) rotate(a, c, p.rope[static_cast<int64_t>(pos) * (D / 2) + j]);
+
+        // Rows of the pool that a tile's positions are in, a position a lane.  Positions past the last one stand for
+        // the last one: their scores are masked, and no lane reads what no position holds.
+        bool bad = false;
+        auto find_rows = [&](int c) {
+            const int x = min(c * kChunk + warp * kTile + (lane & (kTile - 1)), pos);
+            const int n = static_cast<int>(p.page_div.div(x));
+            int page = table[n];
+            if (!paged_valid(page, pc.num_pages)) {
+                bad = true;
+                page = 0;
             }
-            qs[r * S::kQPitch + j] = a;
-            qs[r * S::kQPitch + j + D / 2] = c;
+            return static_cast<uint32_t>((static_cast<int64_t>(page) * pc.kv_heads + kh) * pc.page_size + (x - n * pc.page_size));
+        };
+        uint4 kr[2][S::kKch], vr[4][S::kVch];  // key rows g and g + 8; value rows 2t, 2t + 1, 2t + 8, 2t + 9
+        auto load_k = [&](uint32_t rows) {
+#pragma unroll
+            for (int n = 0; n < 2; ++n) {
+                const uint32_t r = __shfl_sync(0xffffffffu, rows, 8 * n + g);
+                const uint4* src = reinterpret_cast<const uint4*>(kp + static_cast<int64_t>(r) * D) + t;
+#pragma unroll
+                for (int j = 0; j < S::kKch; ++j) kr[n][j] = __ldcg(src + 4 * j);
+            }
+        };
+        auto load_v = [&](uint32_t rows) {
+#pragma unroll
+            for (int n = 0; n < 4; ++n) {
+                const uint32_t r = __shfl_sync(0xffffffffu, rows, 8 * (n >> 1) + 2 * t + (n & 1));
+                const uint4* src = reinterpret_cast<const uint4*>(vp + static_cast<int64_t>(r) * D) + g;
+#pragma unroll
+                for (int j = 0; j < S::kVch; ++j) vr[n][j] = __ldcg(src + 8 * j);
+            }
+        };
+        // The first tile is on its way before the queries are made, unless it holds the position to be written here.
+        const uint32_t rows = find_rows(c0);
+        const bool early = c0 * kChunk + (warp + 1) * kTile <= pos;
+        if (early) {
+            load_k(rows);
+            load_v(rows);
         }
+
+        // The rotated queries, each lane's columns of each step, split in hi and lo.  Columns j and j + d/2 are half
+        // the steps apart, so a thread rotates and writes two steps.
+        if constexpr (kScaled<C>) {
+            if (threadIdx.x < 16) row_max[threadIdx.x] = 0u;
+            __syncthreads();
+        }
+        constexpr int kItems = S::kHalves * (S::kSteps / 2) * 32;
+        constexpr int kEach = (kItems + 127) / 128;
+        float qa[kEach][S::kPer], qb[kEach][S::kPer];
+#pragma unroll
+        for (int n = 0; n < kEach; ++n) {
+            const int i = threadIdx.x + 128 * n, l = i & 31, st = (i >> 5) % (S::kSteps / 2), half = (i >> 5) / (S::kSteps / 2);
+            const int r = (l >> 2) + 8 * half, e0 = (4 * (st / 2) + (l & 3)) * S::kVec + (st & 1) * S::kPer;
+#pragma unroll
+            for (int k = 0; k < S::kPer; ++k) qa[n][k] = qb[n][k] = 0.0f;
+            if (i < kItems && r < nh) {
+                const int64_t src = qrow + static_cast<int64_t>(h0 + r) * D + e0;
+                load_io_n<S::kPer>(p.qkv, src, p.io, qa[n]);
+                load_io_n<S::kPer>(p.qkv, src + D / 2, p.io, qb[n]);
+                if (p.rope) {
+                    const float4* cs = reinterpret_cast<const float4*>(p.rope + static_cast<int64_t>(pos) * (D / 2) + e0);
+#pragma unroll
+                    for (int k = 0; k < S::kPer; k += 2) {
+                        const float4 x = cs[k / 2];
+                        rotate(qa[n][k], qb[n][k], make_float2(x.x, x.y));
+                        rotate(qa[n][k + 1], qb[n][k + 1], make_float2(x.z, x.w));
+                    }
+                }
+                if constexpr (kScaled<C>) {
+                    float big = 0.0f;
+#pragma unroll
+                    for (int k = 0; k < S::kPer; ++k) big = fmaxf(big, fmaxf(fabsf(qa[n][k]), fabsf(qb[n][k])));
+                    atomicMax(&row_max[r], __float_as_uint(big));
+                }
+            }
+        }
+        if constexpr (kScaled<C>) __syncthreads();
+#pragma unroll
+        for (int n = 0; n < kEach; ++n) {
+            const int i = threadIdx.x + 128 * n, l = i & 31, st = (i >> 5) % (S::kSteps / 2), half = (i >> 5) / (S::kSteps / 2);
+            if (i >= kItems) break;
+            float down = 1.0f;
+            if constexpr (kScaled<C>) down = __uint_as_float(static_cast<uint32_t>(127 - row_exponent(row_max[(l >> 2) + 8 * half])) << 23);
+            uint4 *fa = frag + (st * S::kHalves + half) * 32 + l, *fb = fa + (S::kSteps / 2) * S::kHalves * 32;
+            if constexpr (S::k32) {
+                const uint32_t a0 = __float_as_uint(qa[n][0]), a1 = __float_as_uint(qa[n][1]);
+                const uint32_t b0 = __float_as_uint(qb[n][0]), b1 = __float_as_uint(qb[n][1]);
+                *fa = make_uint4(a0, a1, tf32_lo(a0), tf32_lo(a1));
+                *fb = make_uint4(b0, b1, tf32_lo(b0), tf32_lo(b1));
+            } else {
+                uint4 o;
+                split16<C>(qa[n][0] * down, qa[n][1] * down, o.x, o.z);
+                split16<C>(qa[n][S::kPer - 2] * down, qa[n][S::kPer - 1] * down, o.y, o.w);
+                *fa = o;
+                split16<C>(qb[n][0] * down, qb[n][1] * down, o.x, o.z);
+                split16<C>(qb[n][S::kPer - 2] * down, qb[n][S::kPer - 1] * down, o.y, o.w);
+                *fb = o;
+            }
+        }
+        // The CTA that holds the last position writes its key and value.
         if (c1 == nch) {
-            const int page = table[p.page_div.div(pos)];
+            const int n = static_cast<int>(p.page_div.div(pos)), page = table[n];
             if (paged_valid(page, pc.num_pages) && threadIdx.x < D / 2) {
                 const int j = threadIdx.x;
                 const int64_t dst = paged_base(page, kh, pc.kv_heads, pc.page_size, D) +
-                                    static_cast<int64_t>(pos - p.page_div.div(pos) * pc.page_size) * D + j;
+                                    static_cast<int64_t>(pos - n * pc.page_size) * D + j;
                 const int64_t src = qrow + static_cast<int64_t>(p.heads + kh) * D + j, sv = src + static_cast<int64_t>(pc.kv_heads) * D;
                 float a = load_io(p.qkv, src, p.io), c = load_io(p.qkv, src + D / 2, p.io);
                 if (p.rope) rotate(a, c, p.rope[static_cast<int64_t>(pos) * (D / 2) + j]);
@@ -292,192 +449,162 @@ __global__ void __launch_bounds__(128, (AttnShape<C, D, WIDE>::kCtas)) attn_deco
             }
         }
         __syncthreads();  // queries, and the new rows, are there for every warp
-
-        // A lane's part of query rows g and g + 8, scaled to [1, 2) by a power of two.
-        float back[2];  // 2^e log2(e) / sqrt(D): turns a row's products into log2 of its weights
-        uint32_t qh[S::kSteps][4], ql[S::k32 ? 1 : S::kSteps][4];  // fp32: the values themselves
-        {
-            float big[2] = {0.0f, 0.0f};
+        if (!early) {
+            load_k(rows);
+            load_v(rows);
+        }
+        // turn a head's products into log2 of its weights (heads 2t and 2t + 1 of each half)
+        float back[S::kHalves][2];
 #pragma unroll
-            for (int r = 0; r < (WIDE ? 2 : 1); ++r) {
+        for (int h = 0; h < S::kHalves; ++h)
 #pragma unroll
-                for (int j = 0; j < S::kKch; ++j)
-#pragma unroll
-                    for (int i = 0; i < S::kVec; ++i)
-                        big[r] = fmaxf(big[r], fabsf(qs[(g + 8 * r) * S::kQPitch + (4 * j + t) * S::kVec + i]));
-                big[r] = fmaxf(big[r], __shfl_xor_sync(0xffffffffu, big[r], 1));
-                big[r] = fmaxf(big[r], __shfl_xor_sync(0xffffffffu, big[r], 2));
+            for (int j = 0; j < 2; ++j) {
+                back[h][j] = kLog2e / (D == 64 ? 8.0f : 11.313708498984761f);
+                if constexpr (kScaled<C>)
+                    back[h][j] *= __uint_as_float(static_cast<uint32_t>(127 + row_exponent(row_max[8 * h + 2 * t + j])) << 23);
             }
+
+        float top[S::kHalves][2], sum[S::kHalves][2], acc[S::kHalves][D / 16][4];
 #pragma unroll
-            for (int r = 0; r < 2; ++r) {
-                const int e = big[r] > 0.0f && big[r] < 3e38f ? max(-120, min(120, ilogbf(big[r]))) : 0;
-                const float down = __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
-                back[r] = __uint_as_float(static_cast<uint32_t>(127 + e) << 23) * (kLog2e / (D == 64 ? 8.0f : 11.313708498984761f));
-                const float* src = qs + (g + 8 * r) * S::kQPitch;
+        for (int h = 0; h < S::kHalves; ++h) {
+            top[h][0] = top[h][1] = -INFINITY, sum[h][0] = sum[h][1] = 0.0f;
 #pragma unroll
-                for (int s = 0; s < S::kSteps; ++s) {
-                    const int e0 = (4 * (s / 2) + t) * S::kVec + (s & 1) * (S::kVec / 2);
-                    if (!WIDE && r == 1) {
-                        qh[s][1] = qh[s][3] = 0u;
-                        if constexpr (!S::k32) ql[s][1] = ql[s][3] = 0u;
-                    } else if constexpr (S::k32) {
-                        qh[s][r] = __float_as_uint(src[e0] * down);
-                        qh[s][2 + r] = __float_as_uint(src[e0 + 1] * down);
+            for (int i = 0; i < D / 16; ++i)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) acc[h][i][j] = 0.0f;
+        }
+#pragma unroll 1
+        for (int c = c0; c < c1; ++c) {
+            const int x0 = c * kChunk + warp * kTile;
+            if (x0 > pos) break;  // only the last chunk has tiles past the end
+            const uint32_t next = find_rows(c + 1);
+            float s[S::kHalves][4], more[S::kHalves][4];
+#pragma unroll
+            for (int h = 0; h < S::kHalves; ++h)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) s[h][j] = more[h][j] = 0.0f;
+#pragma unroll
+            for (int i = 0; i < S::kSteps; ++i) {
+                const int w = (i & 1) * 2;
+                const uint32_t a[4] = {word(kr[0][i / 2], w), word(kr[1][i / 2], w), word(kr[0][i / 2], w + 1), word(kr[1][i / 2], w + 1)};
+#pragma unroll
+                for (int h = 0; h < S::kHalves; ++h) {
+                    const uint4 q = load_shared(frag + (i * S::kHalves + h) * 32 + lane);
+                    if constexpr (S::k32) {
+                        const uint32_t lo[4] = {tf32_lo(a[0]), tf32_lo(a[1]), tf32_lo(a[2]), tf32_lo(a[3])};
+                        mma_tf32(s[h], a, q.x, q.y);
+                        mma_tf32(more[h], a, q.z, q.w);
+                        mma_tf32(more[h], lo, q.x, q.y);
                     } else {
-                        split16<C>(src[e0] * down, src[e0 + 1] * down, qh[s][r], ql[s][r]);
-                        split16<C>(src[e0 + 2] * down, src[e0 + 3] * down, qh[s][2 + r], ql[s][2 + r]);
+                        mma16(s[h], a, q.x, q.y, C{});
+                        mma16(more[h], a, q.z, q.w, C{});
                     }
                 }
             }
-        }
-
-        float top[2] = {-INFINITY, -INFINITY}, sum[2] = {0.0f, 0.0f};
-        constexpr int kAcc = WIDE ? 4 : 2;  // of an MMA's four results; rows 8 .. 15 are zeros that nobody keeps
-        float acc[D / 8][kAcc];
-#pragma unroll
-        for (int i = 0; i < D / 8; ++i)
-#pragma unroll
-            for (int j = 0; j < kAcc; ++j) acc[i][j] = 0.0f;
-        bool bad = false;
-
-        // Rows of the pool that a tile's positions are in, a position a lane.
-        auto find_rows = [&](int c) {
-            const int x = c * S::kChunk + warp * S::kTile + (lane & (S::kTile - 1));
-            if (c >= c1 || x > pos) return kNoRow;
-            const int n = static_cast<int>(p.page_div.div(x));
-            const int page = table[n];
-            if (!paged_valid(page, pc.num_pages)) {
-                bad = true;
-                return kNoRow;
-            }
-            return static_cast<uint32_t>((static_cast<int64_t>(page) * pc.kv_heads + kh) * pc.page_size + (x - n * pc.page_size));
-        };
-        uint4 kr[S::kNT][S::kKch], vr[2 * S::kNT][S::kVch];
-        const uint4 zero = make_uint4(0u, 0u, 0u, 0u);
-        auto load_k = [&](uint32_t rows) {
-#pragma unroll
-            for (int n = 0; n < S::kNT; ++n) {
-                const uint32_t r = __shfl_sync(0xffffffffu, rows, 8 * n + g);
-                const uint4* src = reinterpret_cast<const uint4*>(kp + static_cast<int64_t>(r) * D) + t;
-#pragma unroll
-                for (int j = 0; j < S::kKch; ++j) kr[n][j] = r == kNoRow ? zero : __ldcg(src + 4 * j);
-            }
-        };
-        auto load_v = [&](uint32_t rows) {
-#pragma unroll
-            for (int n = 0; n < 2 * S::kNT; ++n) {
-                const uint32_t r = __shfl_sync(0xffffffffu, rows, 8 * (n >> 1) + 2 * t + (n & 1));
-                const uint4* src = reinterpret_cast<const uint4*>(vp + static_cast<int64_t>(r) * D) + g;
-#pragma unroll
-                for (int j = 0; j < S::kVch; ++j) vr[n][j] = r == kNoRow ? zero : __ldcg(src + 8 * j);
-            }
-        };
-        uint32_t rows = find_rows(c0);
-        load_k(rows);
-        load_v(rows);
-        for (int c = c0; c < c1; ++c) {
-            const int x0 = c * S::kChunk + warp * S::kTile;
-            const uint32_t next = find_rows(c + 1);
-            if (x0 > pos) break;  // only the last chunk has tiles past the end
-            float s[S::kNT][4];
-#pragma unroll
-            for (int n = 0; n < S::kNT; ++n) {
-#pragma unroll
-                for (int j = 0; j < 4; ++j) s[n][j] = 0.0f;
-#pragma unroll
-                for (int i = 0; i < S::kSteps; ++i) {
-                    const uint32_t b0 = word(kr[n][i / 2], (i & 1) * 2), b1 = word(kr[n][i / 2], (i & 1) * 2 + 1);
-                    if constexpr (S::k32) mma_split3(s[n], qh[i], b0, b1);
-                    else mma_split<C>(s[n], qh[i], ql[i], b0, b1);
-                }
-            }
             load_k(next);
-            float high[2] = {-INFINITY, -INFINITY};
+            float old[S::kHalves][2];
+            bool raise = false;
 #pragma unroll
-            for (int n = 0; n < S::kNT; ++n)
+            for (int h = 0; h < S::kHalves; ++h) {
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    s[n][j] = x0 + 8 * n + 2 * t + (j & 1) <= pos ? s[n][j] * back[j >> 1] : -INFINITY;
-                    if (WIDE || j < 2) high[j >> 1] = fmaxf(high[j >> 1], s[n][j]);
-                }
-            float old[2] = {1.0f, 1.0f};
-#pragma unroll
-            for (int r = 0; r < (WIDE ? 2 : 1); ++r) {
-                high[r] = fmaxf(high[r], __shfl_xor_sync(0xffffffffu, high[r], 1));
-                high[r] = fmaxf(high[r], __shfl_xor_sync(0xffffffffu, high[r], 2));
-                high[r] = fmaxf(high[r], top[r]);
-                old[r] = exp2f(top[r] - high[r]);
-                top[r] = high[r];
-                sum[r] *= old[r];
-            }
-            if (__any_sync(0xffffffffu, old[0] != 1.0f || old[1] != 1.0f)) {
-#pragma unroll
-                for (int i = 0; i < D / 8; ++i)
-#pragma unroll
-                    for (int j = 0; j < kAcc; ++j) acc[i][j] *= old[j >> 1];
-            }
-            uint32_t wh[S::kNT][4], wl[S::kNT][4];
-#pragma unroll
-            for (int n = 0; n < S::kNT; ++n) {
-#pragma unroll
-                for (int j = 0; j < (WIDE ? 4 : 2); ++j) {
-                    s[n][j] = exp2f(s[n][j] - top[j >> 1]);
-                    sum[j >> 1] += s[n][j];
-                }
-                if (!WIDE) s[n][2] = s[n][3] = 0.0f;
-            }
-            if constexpr (S::k32) {
-                // position 2t is the MMA's k = t, 2t + 1 its k = t + 4
-#pragma unroll
-                for (int n = 0; n < S::kNT; ++n)
+                for (int j = 0; j < 4; ++j) s[h][j] = (s[h][j] + more[h][j]) * back[h][j & 1];
+                if (x0 + kTile > pos + 1) {
 #pragma unroll
                     for (int j = 0; j < 4; ++j)
-                        wh[n][j] = __float_as_uint(s[n][(j & 1) * 2 + (j >> 1)]);
-#pragma unroll
-                for (int i = 0; i < D / 8; ++i) {
-                    float o[4] = {acc[i][0], acc[i][1], WIDE ? acc[i][kAcc - 2] : 0.0f, WIDE ? acc[i][kAcc - 1] : 0.0f};
-#pragma unroll
-                    for (int n = 0; n < S::kNT; ++n)
-                        mma_split3(o, wh[n], word(vr[2 * n][i / S::kVec], i % S::kVec),
-                                   word(vr[2 * n + 1][i / S::kVec], i % S::kVec));
-#pragma unroll
-                    for (int j = 0; j < kAcc; ++j) acc[i][j] = o[j];
+                        if (x0 + g + (j >> 1) * 8 > pos) s[h][j] = -INFINITY;
                 }
-            } else {
-                split16<C>(s[0][0], s[0][1], wh[0][0], wl[0][0]);
-                split16<C>(s[0][2], s[0][3], wh[0][1], wl[0][1]);
-                split16<C>(s[S::kNT - 1][0], s[S::kNT - 1][1], wh[0][2], wl[0][2]);
-                split16<C>(s[S::kNT - 1][2], s[S::kNT - 1][3], wh[0][3], wl[0][3]);
 #pragma unroll
-                for (int i = 0; i < D / 8; ++i) {
-                    const int ch = i / S::kVec, e = i % S::kVec;
-                    const uint32_t pick = e & 1 ? 0x7632u : 0x5410u;
-                    const uint32_t b0 = __byte_perm(word(vr[0][ch], e / 2), word(vr[1][ch], e / 2), pick);
-                    const uint32_t b1 = __byte_perm(word(vr[2 * S::kNT - 2][ch], e / 2), word(vr[2 * S::kNT - 1][ch], e / 2), pick);
-                    float o[4] = {acc[i][0], acc[i][1], WIDE ? acc[i][kAcc - 2] : 0.0f, WIDE ? acc[i][kAcc - 1] : 0.0f};
-                    mma_split<C>(o, wh[0], wl[0], b0, b1);
+                for (int j = 0; j < 2; ++j) {
+                    float high = fmaxf(s[h][j], s[h][j + 2]);
+                    high = fmaxf(high, __shfl_xor_sync(0xffffffffu, high, 4));
+                    high = fmaxf(high, __shfl_xor_sync(0xffffffffu, high, 8));
+                    high = fmaxf(high, __shfl_xor_sync(0xffffffffu, high, 16));
+                    high = fmaxf(high, top[h][j]);
+                    old[h][j] = exp2_fast(top[h][j] - high);
+                    raise |= high != top[h][j];
+                    top[h][j] = high;
+                    s[h][j] = exp2_fast(s[h][j] - high);
+                    s[h][j + 2] = exp2_fast(s[h][j + 2] - high);
+                    sum[h][j] = sum[h][j] * old[h][j] + (s[h][j] + s[h][j + 2]);
+                }
+            }
+            if (__any_sync(0xffffffffu, raise)) {
 #pragma unroll
-                    for (int j = 0; j < kAcc; ++j) acc[i][j] = o[j];
+                for (int h = 0; h < S::kHalves; ++h)
+#pragma unroll
+                    for (int i = 0; i < D / 16; ++i)
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) acc[h][i][j] *= old[h][j & 1];
+            }
+            // The weights as the next MMAs' second operand: head g, positions 2t, 2t + 1 and those + 8.
+            uint32_t wh[S::kHalves][4], wl[S::kHalves][4];
+#pragma unroll
+            for (int h = 0; h < S::kHalves; ++h)
+#pragma unroll
+                for (int n = 0; n < 2; ++n) {
+                    if constexpr (S::k32) {
+                        const uint32_t x = __float_as_uint(s[h][2 * n]), y = __float_as_uint(s[h][2 * n + 1]);
+                        const uint32_t up = transpose8(__byte_perm(x, y, 0x7632)), down = transpose8(__byte_perm(x, y, 0x5410));
+                        wh[h][2 * n] = __byte_perm(down, up, 0x5410);
+                        wh[h][2 * n + 1] = __byte_perm(down, up, 0x7632);
+                        wl[h][2 * n] = tf32_lo(wh[h][2 * n]), wl[h][2 * n + 1] = tf32_lo(wh[h][2 * n + 1]);
+                    } else {
+                        uint32_t hi, lo;
+                        split16<C>(s[h][2 * n], s[h][2 * n + 1], hi, lo);
+                        wh[h][n] = transpose8(hi), wl[h][n] = transpose8(lo);
+                    }
+                }
+#pragma unroll
+            for (int i = 0; i < D / 16; ++i) {
+                const int ch = i / (S::kVec / 2), e = i % (S::kVec / 2);
+                if constexpr (S::k32) {
+                    // position 2t is the MMA's k = t, 2t + 1 its k = t + 4; columns 2e and 2e + 1 its rows g and g + 8
+#pragma unroll
+                    for (int n = 0; n < 2; ++n) {
+                        const uint32_t a[4] = {word(vr[2 * n][ch], 2 * e), word(vr[2 * n][ch], 2 * e + 1),
+                                               word(vr[2 * n + 1][ch], 2 * e), word(vr[2 * n + 1][ch], 2 * e + 1)};
+                        const uint32_t lo[4] = {tf32_lo(a[0]), tf32_lo(a[1]), tf32_lo(a[2]), tf32_lo(a[3])};
+#pragma unroll
+                        for (int h = 0; h < S::kHalves; ++h) {
+                            mma_tf32(acc[h][i], a, wh[h][2 * n], wh[h][2 * n + 1]);
+                            mma_tf32(acc[h][i], a, wl[h][2 * n], wl[h][2 * n + 1]);
+                            mma_tf32(acc[h][i], lo, wh[h][2 * n], wh[h][2 * n + 1]);
+                        }
+                    }
+                } else {
+                    const uint32_t x = word(vr[0][ch], e), y = word(vr[1][ch], e), z = word(vr[2][ch], e), u = word(vr[3][ch], e);
+                    const uint32_t a[4] = {__byte_perm(x, y, 0x5410), __byte_perm(x, y, 0x7632), __byte_perm(z, u, 0x5410),
+                                           __byte_perm(z, u, 0x7632)};
+#pragma unroll
+                    for (int h = 0; h < S::kHalves; ++h) {
+                        mma16(acc[h][i], a, wh[h][0], wh[h][1], C{});
+                        mma16(acc[h][i], a, wl[h][0], wl[h][1], C{});
+                    }
                 }
             }
             load_v(next);
         }
 
+        __syncthreads();  // the queries have been read
         // The warps' rows: output parts, then maximum and sum.
+        bad = __any_sync(0xffffffffu, bad);
 #pragma unroll
-        for (int r = 0; r < (WIDE ? 2 : 1); ++r) {
-            sum[r] += __shfl_xor_sync(0xffffffffu, sum[r], 1);
-            sum[r] += __shfl_xor_sync(0xffffffffu, sum[r], 2);
-            float* row = warp_part + (warp * S::kRows + g + 8 * r) * (D + 2);
+        for (int h = 0; h < S::kHalves; ++h)
 #pragma unroll
-            for (int i = 0; i < D / 8; ++i) {
-                const int d = (i / S::kVec) * 8 * S::kVec + 2 * t * S::kVec + i % S::kVec;
-                row[d] = acc[i][(2 * r) % kAcc];
-                row[d + S::kVec] = acc[i][(2 * r + 1) % kAcc];
+            for (int j = 0; j < 2; ++j) {
+                float l = sum[h][j];
+#pragma unroll
+                for (int o = 4; o < 32; o <<= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
+                if (bad) l = __int_as_float(0x7fffffff);
+                float* row = warp_part + (warp * S::kRows + 8 * h + 2 * t + j) * (D + 2);
+#pragma unroll
+                for (int i = 0; i < D / 16; ++i) {
+                    const int d = (i / (S::kVec / 2)) * 8 * S::kVec + S::kVec * g + 2 * (i % (S::kVec / 2));
+                    row[d] = acc[h][i][j];
+                    row[d + 1] = acc[h][i][j + 2];
+                }
+                if (g == 0) row[D] = top[h][j], row[D + 1] = l;
             }
-            if (__any_sync(0xffffffffu, bad)) sum[r] = __int_as_float(0x7fffffff);
-            if (t == 0) row[D] = top[r], row[D + 1] = sum[r];
-        }
         __syncthreads();
         const bool whole = c0 == 0 && c1 == nch;
         const int slot = 2 * blockIdx.x + (c0 > 0 ? 0 : 1);
@@ -506,7 +633,7 @@ __global__ void __launch_bounds__(128, (AttnShape<C, D, WIDE>::kCtas)) attn_deco
 
         // The pair's last CTA to come here merges all its partials, in CTA order.
         const int cta0 = static_cast<int>(((pair_first + 1) * grid - 1) / all);
-        const int cta1 = static_cast<int>(((pair_first + nch) * grid - 1) / all);
+        const int cta1 = static_cast<int>(((pair_first + nu) * grid - 1) / all);
         int* ticket = p.tickets + static_cast<int64_t>(seq) * pairs + pair;
         __threadfence();
         __syncthreads();
@@ -514,22 +641,49 @@ __global__ void __launch_bounds__(128, (AttnShape<C, D, WIDE>::kCtas)) attn_deco
         __syncthreads();
         if (!flag) continue;
         __threadfence();
-        for (int i = threadIdx.x; i < nh * D; i += 128) {
-            const int r = i / D, d = i - r * D;
-            float m = -INFINITY, l = 0.0f, o = 0.0f;
-            for (int c = cta0; c <= cta1; ++c) {
-                // a pair begins within its first CTA's stretch unless that stretch begins with it
-                const int sl = 2 * c + (c == cta0 ? 1 : 0);
-                const float* x = p.part + sl * static_cast<int64_t>(S::kRows * (D + 2)) + r * (D + 2);
-                const float xm = __ldcg(x + D), xl = __ldcg(x + D + 1), xo = __ldcg(x + d);
-                const float up = fmaxf(m, xm);
-                const float f0 = m == -INFINITY ? 0.0f : exp2f(m - up), f1 = xm == -INFINITY ? 0.0f : exp2f(xm - up);
-                l = l * f0 + xl * f1;
-                if (xl != xl) l = xl;
-                o = o * f0 + xo * f1;
-                m = up;
+        // A warp a head, 4 columns a lane (d = 64: half a warp takes every other partial), kMergeAhead partials in
+        // flight: a long sequence alone has dozens of them, and one at a time would cost a memory round trip each.
+        constexpr int kLanes = D / 4, kApart = 32 / kLanes;
+        for (int r = warp; r < nh; r += kAttnWarps) {
+            float m = -INFINITY, l = 0.0f, o[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+            const int d = (lane % kLanes) * 4;
+            for (int c = cta0; c <= cta1; c += kMergeAhead * kApart) {
+                float2 ml[kMergeAhead];
+                float2 x[kMergeAhead][2];
+#pragma unroll
+                for (int k = 0; k < kMergeAhead; ++k) {
+                    const int from = c + k * kApart + lane / kLanes;
+                    // a pair's first CTA leaves it in the second slot: its stretch ends with the pair's beginning
+                    const float* src = p.part + (2 * min(from, cta1) + (min(from, cta1) == cta0 ? 1 : 0)) *
+                                                    static_cast<int64_t>(S::kRows * (D + 2)) + r * (D + 2);
+                    ml[k] = __ldcg(reinterpret_cast<const float2*>(src + D));
+                    x[k][0] = __ldcg(reinterpret_cast<const float2*>(src + d));
+                    x[k][1] = __ldcg(reinterpret_cast<const float2*>(src + d + 2));
+                    if (from > cta1) ml[k] = make_float2(-INFINITY, 0.0f);
+                }
+#pragma unroll
+                for (int k = 0; k < kMergeAhead; ++k) {
+                    const float up = fmaxf(m, ml[k].x);
+                    const float f0 = m == -INFINITY ? 0.0f : exp2_fast(m - up);
+                    const float f1 = ml[k].x == -INFINITY ? 0.0f : exp2_fast(ml[k].x - up);
+                    l = ml[k].y != ml[k].y ? ml[k].y : l * f0 + ml[k].y * f1;
+                    o[0] = o[0] * f0 + x[k][0].x * f1, o[1] = o[1] * f0 + x[k][0].y * f1;
+                    o[2] = o[2] * f0 + x[k][1].x * f1, o[3] = o[3] * f0 + x[k][1].y * f1;
+                    m = up;
+                }
             }
-            store_io(p.out, out0 + i, o / l, p.io);
+            if (kApart == 2) {
+                const float m2 = __shfl_xor_sync(0xffffffffu, m, 16), l2 = __shfl_xor_sync(0xffffffffu, l, 16);
+                const float up = fmaxf(m, m2);
+                const float f0 = m == -INFINITY ? 0.0f : exp2_fast(m - up), f1 = m2 == -INFINITY ? 0.0f : exp2_fast(m2 - up);
+                l = l != l || l2 != l2 ? __int_as_float(0x7fffffff) : l * f0 + l2 * f1;
+#pragma unroll
+                for (int k = 0; k < 4; ++k) o[k] = o[k] * f0 + __shfl_xor_sync(0xffffffffu, o[k], 16) * f1;
+            }
+            if (lane < kLanes) {
+#pragma unroll
+                for (int k = 0; k < 4; ++k) store_io(p.out, out0 + r * D + d + k, o[k] / l, p.io);
+            }
         }
         if (threadIdx.x == 0) *ticket = 0;
     }
@@ -552,7 +706,7 @@ cudaError_t attend_shape(AttnParams p, int num_sms, cudaStream_t s) {
     using S = AttnShape<C, D, WIDE>;
     p.blocks = (p.group - 1) / S::kRows + 1;
     const long long longest = static_cast<long long>(p.pc.max_pages) * p.pc.page_size;
-    const long long chunks = ((longest - 1) / S::kChunk + 1) * p.pc.batch * p.pc.kv_heads * p.blocks;
+    const long long chunks = ((longest - 1) / kChunk + 1) * p.pc.batch * p.pc.kv_heads * p.blocks;
     const long long most = std::min(num_sms * S::kCtas, kAttnMaxCtas);
     count_launch();
     attn_decode_paged_kernel<C, D, WIDE>
