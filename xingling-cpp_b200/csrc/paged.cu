@@ -259,14 +259,10 @@ __global__ void __launch_bounds__(128, (AttnShape<C, D, WIDE>::kCtas)) attn_deco
     // finds the sequence that its CTA's stretch begins in; the positions are read once where a warp holds them all.
     const int held = lane < pc.batch ? chunks_of(p.pos[lane]) : 0;
     auto chunks_at = [&](int i) { return i < 32 ? held : i < pc.batch ? chunks_of(p.pos[i]) : 0; };
-    auto units_in_all = [&](int step) {
-        long long total = 0;
-        for (int b0 = 0; b0 < pc.batch; b0 += 32) {
-            long long c = (chunks_at(b0 + lane) + step - 1) / step;
-#pragma unroll
-            for (int o = 16; o; o >>= 1) c += __shfl_xor_sync(0xffffffffu, c, o);
-            total += c;
-        }
+    auto units_in_all = [&](unsigned step) {
+        long long total = 0;  // a sequence has at most 2^25 chunks, 32 of them fit 32 bits
+        for (int b0 = 0; b0 < pc.batch; b0 += 32)
+            total += __reduce_add_sync(0xffffffffu, static_cast<unsigned>(chunks_at(b0 + lane) + step - 1) / step);
         return total * pairs;
     };
     // Short work: the step is raised until every CTA has one unit at most, so that none takes parts of two pairs one
@@ -285,32 +281,37 @@ __global__ void __launch_bounds__(128, (AttnShape<C, D, WIDE>::kCtas)) attn_deco
     }
     const long long grid = min(static_cast<long long>(gridDim.x), all);  // a unit at least for every CTA that works
     if (blockIdx.x >= grid) return;
-    long long at = blockIdx.x * all / grid;
-    const long long end = (blockIdx.x + 1) * all / grid;
+    // (64-bit divisions take hundreds of clocks: 32 bits where they do)
+    const bool brief = all < (1ll << 31) / kAttnMaxCtas;
+    auto share = [&](unsigned i) {
+        return brief ? static_cast<long long>(i * static_cast<unsigned>(all) / static_cast<unsigned>(grid)) : i * all / grid;
+    };
+    long long at = share(blockIdx.x);
+    const long long end = share(blockIdx.x + 1);
     int b = 0;
     long long first = 0;  // the row's index of sequence b's first unit
     for (int b0 = 0; b0 < pc.batch; b0 += 32) {
-        const long long own = static_cast<long long>((chunks_at(b0 + lane) + step - 1) / step) * pairs;
-        long long upto = own;
+        const unsigned own = static_cast<unsigned>(chunks_at(b0 + lane) + step - 1) / static_cast<unsigned>(step);
+        unsigned upto = own;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
-            const long long v = __shfl_up_sync(0xffffffffu, upto, o);
+            const unsigned v = __shfl_up_sync(0xffffffffu, upto, o);
             if (lane >= o) upto += v;
         }
-        const uint32_t past = __ballot_sync(0xffffffffu, first + upto > at);
+        const uint32_t past = __ballot_sync(0xffffffffu, first + static_cast<long long>(upto) * pairs > at);
         if (past) {
             const int i = __ffs(past) - 1;
             b = b0 + i;
-            first += __shfl_sync(0xffffffffu, upto - own, i);
+            first += static_cast<long long>(__shfl_sync(0xffffffffu, upto - own, i)) * pairs;
             break;
         }
-        first += __shfl_sync(0xffffffffu, upto, 31);
+        first += static_cast<long long>(__shfl_sync(0xffffffffu, upto, 31)) * pairs;
     }
 
     while (at < end) {
         const int pos = p.pos[b];
         const int nch = chunks_of(pos), nu = (nch + step - 1) / step;
-        const int pair = static_cast<int>((at - first) / nu);
+        const int pair = brief ? static_cast<int>(at - first) / nu : static_cast<int>((at - first) / nu);
         const int u0 = static_cast<int>((at - first) - static_cast<long long>(pair) * nu);
         const int u1 = static_cast<int>(min(static_cast<long long>(nu), u0 + (end - at)));
         const int c0 = u0 * step, c1 = min(nch, u1 * step);
@@ -374,6 +375,20 @@ __global__ void __launch_bounds__(128, (AttnShape<C, D, WIDE>::kCtas)) attn_deco
             load_v(rows);
         }
 
+        // The CTA that holds the last position writes its key and value (read here, written when the queries are made).
+        int64_t new_at = -1;
+        float new_row[4];
+        float2 new_cs = make_float2(1.0f, 0.0f);
+        if (c1 == nch && threadIdx.x < D / 2) {
+            const int n = static_cast<int>(p.page_div.div(pos)), page = table[n], j = threadIdx.x;
+            const int64_t src = qrow + static_cast<int64_t>(p.heads + kh) * D + j, sv = src + static_cast<int64_t>(pc.kv_heads) * D;
+            new_row[0] = load_io(p.qkv, src, p.io), new_row[1] = load_io(p.qkv, src + D / 2, p.io);
+            new_row[2] = load_io(p.qkv, sv, p.io), new_row[3] = load_io(p.qkv, sv + D / 2, p.io);
+            if (p.rope) new_cs = p.rope[static_cast<int64_t>(pos) * (D / 2) + j];
+            if (paged_valid(page, pc.num_pages))
+                new_at = paged_base(page, kh, pc.kv_heads, pc.page_size, D) + static_cast<int64_t>(pos - n * pc.page_size) * D + j;
+        }
+
         // The rotated queries, each lane's columns of each step, split in hi and lo.  Columns j and j + d/2 are half
         // the steps apart, so a thread rotates and writes two steps.
         if constexpr (kScaled<C>) {
@@ -433,20 +448,10 @@ __global__ void __launch_bounds__(128, (AttnShape<C, D, WIDE>::kCtas)) attn_deco
                 *fb = o;
             }
         }
-        // The CTA that holds the last position writes its key and value.
-        if (c1 == nch) {
-            const int n = static_cast<int>(p.page_div.div(pos)), page = table[n];
-            if (paged_valid(page, pc.num_pages) && threadIdx.x < D / 2) {
-                const int j = threadIdx.x;
-                const int64_t dst = paged_base(page, kh, pc.kv_heads, pc.page_size, D) +
-                                    static_cast<int64_t>(pos - n * pc.page_size) * D + j;
-                const int64_t src = qrow + static_cast<int64_t>(p.heads + kh) * D + j, sv = src + static_cast<int64_t>(pc.kv_heads) * D;
-                float a = load_io(p.qkv, src, p.io), c = load_io(p.qkv, src + D / 2, p.io);
-                if (p.rope) rotate(a, c, p.rope[static_cast<int64_t>(pos) * (D / 2) + j]);
-                kp[dst] = from_float<C>(a), kp[dst + D / 2] = from_float<C>(c);
-                vp[dst] = from_float<C>(load_io(p.qkv, sv, p.io));
-                vp[dst + D / 2] = from_float<C>(load_io(p.qkv, sv + D / 2, p.io));
-            }
+        if (new_at >= 0) {
+            if (p.rope) rotate(new_row[0], new_row[1], new_cs);
+            kp[new_at] = from_float<C>(new_row[0]), kp[new_at + D / 2] = from_float<C>(new_row[1]);
+            vp[new_at] = from_float<C>(new_row[2]), vp[new_at + D / 2] = from_float<C>(new_row[3]);
         }
         __syncthreads();  // queries, and the new rows, are there for every warp
         if (!early) {
@@ -632,15 +637,20 @@ __global__ void __launch_bounds__(128, (AttnShape<C, D, WIDE>::kCtas)) attn_deco
         if (whole) continue;
 
         // The pair's last CTA to come here merges all its partials, in CTA order.
-        const int cta0 = static_cast<int>(((pair_first + 1) * grid - 1) / all);
-        const int cta1 = static_cast<int>(((pair_first + nu) * grid - 1) / all);
+        auto owner = [&](long long unit) {
+            const long long v = (unit + 1) * grid - 1;
+            return brief ? static_cast<int>(static_cast<unsigned>(v) / static_cast<unsigned>(all)) : static_cast<int>(v / all);
+        };
+        const int cta0 = owner(pair_first), cta1 = owner(pair_first + nu - 1);
         int* ticket = p.tickets + static_cast<int64_t>(seq) * pairs + pair;
-        __threadfence();
-        __syncthreads();
-        if (threadIdx.x == 0) flag = atomicAdd(ticket, 1) == cta1 - cta0;
+        __syncthreads();  // the partial is written; one thread's fence carries it to the others' reads
+        if (threadIdx.x == 0) {
+            __threadfence();
+            flag = atomicAdd(ticket, 1) == cta1 - cta0;
+            __threadfence();
+        }
         __syncthreads();
         if (!flag) continue;
-        __threadfence();
         // A warp a head, 4 columns a lane (d = 64: half a warp takes every other partial), kMergeAhead partials in
         // flight: a long sequence alone has dozens of them, and one at a time would cost a memory round trip each.
         constexpr int kLanes = D / 4, kApart = 32 / kLanes;
