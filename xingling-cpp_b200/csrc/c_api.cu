@@ -558,7 +558,7 @@ int xl_op_add_rmsnorm_fp8(int dtype, const void* delta, const void* residual, vo
     int sms = 0;
     const int rc = on_current_device(op, {delta, residual, delta ? residual_out : nullptr, gamma, q, scale}, &sms);
     if (rc != XL_OK) return rc;
-    return cuda_status(xl::launch_add_rmsnorm_fp8(dtype, delta, residual, residual_out, gamma, q, ldq, scale, n, k,
+    return cuda_status(xl::launch_add_rmsnorm_fp8(dtype, delta, residual, residual_out, gamma, q, ldq, scale, n, k, sms,
                                                   as_stream(stream)), op);
 }
 

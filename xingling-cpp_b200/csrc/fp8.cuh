@@ -50,15 +50,35 @@ __device__ __forceinline__ void store8(T* p, const float (&v)[8]) {
         *reinterpret_cast<uint4*>(p) = u;
     }
 }
-// The first `live` of 8 consecutive elements (0 for the others); `vec`: the address is 16-byte aligned.
+// 8 elements as they lie in memory, so that several loads can be under way before the first is converted.
 template <typename T>
-__device__ __forceinline__ void load8_ragged(const T* p, int live, bool vec, float (&v)[8]) {
-    if (vec && live >= 8) {
-        load8(p, v);
-    } else {
+struct Raw8 {
+    uint4 w[sizeof(T) / 2];
+};
+// VEC: all 8 (a 16-byte aligned address) or, with live 0, zeros.  Else the first `live`, zeros for the others.
+template <bool VEC, typename T>
+__device__ __forceinline__ Raw8<T> load_raw8(const T* p, int live) {
+    Raw8<T> r;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = i < live ? to_float(p[i]) : 0.0f;
+    for (int i = 0; i < static_cast<int>(sizeof(T) / 2); ++i) r.w[i] = make_uint4(0u, 0u, 0u, 0u);
+    if constexpr (VEC) {
+        if (live) {
+#pragma unroll
+            for (int i = 0; i < static_cast<int>(sizeof(T) / 2); ++i) r.w[i] = reinterpret_cast<const uint4*>(p)[i];
+        }
+    } else {
+        T* e = reinterpret_cast<T*>(&r);
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            if (i < live) e[i] = p[i];
     }
+    return r;
+}
+template <typename T>
+__device__ __forceinline__ void to_floats(const Raw8<T>& r, float (&v)[8]) {
+    const T* e = reinterpret_cast<const T*>(&r);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = to_float(e[i]);
 }
 
 // Two floats to two e4m3 bytes (the first in the low byte), to nearest, ties to even; NaN stays NaN.
@@ -79,13 +99,14 @@ __device__ __forceinline__ uint32_t e4m3_of(double v) {
 
 // Whether a 32-bit quotient that is at most 8 units in the last place off may
 // lie on the other side of a border between two e4m3 values than the exact
-// one does.  Borders are where the 4th bit after the leading one is set and
-// nothing follows; below 2^-6 (steps of 2^-9) the odd multiples of 2^-10.
-__device__ __forceinline__ bool near_border(float q) {
-    const uint32_t u = __float_as_uint(q) & 0x7fffffffu;
-    if (u >= 0x3c800000u) return ((u - 0x7fff8u) & 0xfffffu) <= 16u;
-    const float m = __uint_as_float(u) * 1024.0f, r = rintf(m);
-    return fabsf(m - r) < 1e-5f && (static_cast<int>(r) & 1);
+// one does.  From 2^-6 on borders are where the 4th bit after the leading one
+// is set and nothing follows; below (steps of 2^-9) the odd multiples of 2^-10.
+__device__ __forceinline__ bool near_border_normal(float q) {
+    return ((__float_as_uint(q) - 0x7fff8u) & 0xfffffu) <= 16u;
+}
+__device__ __forceinline__ bool near_border_small(float q) {
+    const float m = fabsf(q) * 1024.0f, r = rintf(m);
+    return m <= 16.0f && fabsf(m - r) < 1e-5f && (static_cast<int>(r) & 1);
 }
 
 // n / d for 0 <= n < 2^31 with a multiplication (Granlund and Montgomery,

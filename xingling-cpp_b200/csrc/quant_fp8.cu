@@ -34,19 +34,24 @@ __device__ __forceinline__ GroupScale group_scale(float s) {
     GroupScale g;
     g.s = s;
     g.exact_only = s > 0.0f && s < 1e-30f;
-    g.inv = s > 0.0f ? 1.0f / s : 0.0f;
+    g.inv = s > 0.0f ? __fdividef(1.0f, s) : 0.0f;  // within 2 ulp: s is below 2^126
     return g;
 }
 
 // Bytes of 8 quotients; y(i) is the exact value in 64 bits, fast(i) its quotient by the scale in 32.
 template <typename Fast, typename Exact>
 __device__ __forceinline__ uint2 quantise8(const GroupScale& g, Fast fast, Exact y) {
-    float q[8];
+    float q[8], least = INFINITY;
     bool close = g.exact_only;
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
         q[i] = fast(i);
-        close |= near_border(q[i]);
+        close |= near_border_normal(q[i]);
+        least = fminf(least, fabsf(q[i]));
+    }
+    if (least < 0.015625f) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) close |= near_border_small(q[i]);
     }
     uint2 out;
     out.x = e4m3x2(q[0], q[1]) | e4m3x2(q[2], q[3]) << 16;
@@ -93,10 +98,10 @@ __device__ __forceinline__ uint2 quantise_plain(const float (&v)[8], const Group
 }
 
 // One scale per row and 128 columns: 16 lanes a group, 8 columns a lane.
-template <typename T>
+template <typename T, bool VEC>
 __global__ void __launch_bounds__(256) quantize_rows_kernel(const T* __restrict__ x, size_t ldx, uint8_t* __restrict__ q,
                                                             size_t ldq, float* __restrict__ scale, uint32_t groups,
-                                                            FastDiv per_row, int k, bool vec) {
+                                                            FastDiv per_row, int k) {
     const uint32_t stride = gridDim.x * (256 / kLanesPerGroup);
     const int sub = threadIdx.x % kLanesPerGroup;
     // whole warps stay in the loop: the reductions shuffle across the half-warp only, but name the warp
@@ -108,7 +113,7 @@ __global__ void __launch_bounds__(256) quantize_rows_kernel(const T* __restrict_
         const int c = static_cast<int>(gi - row * per_row.d) * kFp8Block + sub * 8;
         const int live = on ? max(0, min(8, k - c)) : 0;
         float v[8];
-        load8_ragged(x + row * ldx + (live ? c : 0), live, vec, v);
+        to_floats(load_raw8<VEC>(x + row * ldx + (live ? c : 0), live), v);
         uint32_t a = 0;
 #pragma unroll
         for (int i = 0; i < 8; ++i) a = umax(a, abs_bits(v[i]));
@@ -123,23 +128,26 @@ __global__ void __launch_bounds__(256) quantize_rows_kernel(const T* __restrict_
 
 // One scale per block of 128 x 128: a CTA keeps the block in registers, so it
 // is read once (64 values a thread, 16 loads of 16 bytes in flight for fp32).
-template <typename T>
+template <typename T, bool VEC>
 __global__ void __launch_bounds__(256) quantize_blocks_kernel(const T* __restrict__ x, size_t ldx, uint8_t* __restrict__ q,
                                                               size_t ldq, float* __restrict__ scale, FastDiv per_row,
-                                                              int n, int k, bool vec) {
+                                                              int n, int k) {
     __shared__ uint32_t red[8];
     const uint32_t rb = per_row.div(blockIdx.x);
     const int c = static_cast<int>(blockIdx.x - rb * per_row.d) * kFp8Block + (threadIdx.x % kLanesPerGroup) * 8;
     const int live = max(0, min(8, k - c));
     const long long r0 = static_cast<long long>(rb) * kFp8Block + threadIdx.x / kLanesPerGroup;
+    Raw8<T> raw[8];
     float v[8][8];
     uint32_t a = 0;
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
         const long long r = r0 + 16 * j;
         const bool on = r < n && live;
-        load8_ragged(x + (on ? r * ldx + c : 0), on ? live : 0, vec, v[j]);
+        raw[j] = load_raw8<VEC>(x + (on ? r * ldx + c : 0), on ? live : 0);
     }
+#pragma unroll
+    for (int j = 0; j < 8; ++j) to_floats(raw[j], v[j]);
 #pragma unroll
     for (int j = 0; j < 8; ++j)
 #pragma unroll
@@ -162,31 +170,42 @@ __global__ void __launch_bounds__(256) quantize_blocks_kernel(const T* __restric
 // r = fl_T(residual + delta) (stored where there is a delta), rs =
 // 1 / sqrt(mean(r^2) + eps), y = r gamma rs, e4m3 per row and 128 columns.
 // One row a CTA, kept in registers (CHUNKS x 8 columns a thread), so each
-// input is read once.  The sum of squares and the products r gamma that set
-// the scales are 64-bit: both are exact or nearly so, so a group's scale and
-// bytes do not depend on the order of the sum.
-template <typename T, int CHUNKS>
-__global__ void __launch_bounds__(1024) add_rmsnorm_fp8_kernel(const T* __restrict__ delta, const T* residual, T* sum,
-                                                               const float* __restrict__ gamma, uint8_t* __restrict__ q,
-                                                               size_t ldq, float* __restrict__ scale, int k, bool vec) {
+// input is read once.  The sum of squares is 64-bit and the largest |r gamma|
+// of a group is found exactly: as the largest fp32 product (rounding keeps the
+// order) and, among those that round to it, the largest remainder.  So a
+// group's scale and bytes do not depend on the order of the sum.
+template <typename T, int CHUNKS, int THREADS, bool VEC>
+__global__ void __launch_bounds__(THREADS) add_rmsnorm_fp8_kernel(const T* __restrict__ delta, const T* residual, T* sum,
+                                                                  const float* __restrict__ gamma,
+                                                                  uint8_t* __restrict__ q, size_t ldq,
+                                                                  float* __restrict__ scale, int k) {
     __shared__ double red[32];
     const size_t row = blockIdx.x;
     const int warp = threadIdx.x >> 5;
-    float r[CHUNKS][8];
-    double ss = 0.0;
+    Raw8<T> raw_r[CHUNKS], raw_d[CHUNKS];
 #pragma unroll
     for (int j = 0; j < CHUNKS; ++j) {
         const int c = static_cast<int>(threadIdx.x + j * blockDim.x) * 8;
         const int live = max(0, min(8, k - c));
         const size_t at = row * k + (live ? c : 0);
-        load8_ragged(residual + at, live, vec, r[j]);
+        raw_r[j] = load_raw8<VEC>(residual + at, live);
+        raw_d[j] = load_raw8<VEC>(delta + at, delta ? live : 0);
+    }
+    float r[CHUNKS][8];
+    double ss = 0.0;
+#pragma unroll
+    for (int j = 0; j < CHUNKS; ++j) {
+        to_floats(raw_r[j], r[j]);
         if (delta) {
+            const int c = static_cast<int>(threadIdx.x + j * blockDim.x) * 8;
+            const int live = max(0, min(8, k - c));
+            const size_t at = row * k + (live ? c : 0);
             float d[8];
-            load8_ragged(delta + at, live, vec, d);
+            to_floats(raw_d[j], d);
 #pragma unroll
             for (int i = 0; i < 8; ++i) r[j][i] = to_float(from_float<T>(r[j][i] + d[i]));
-            if (vec && live == 8) {
-                store8(sum + at, r[j]);
+            if (VEC) {
+                if (live) store8(sum + at, r[j]);
             } else {
 #pragma unroll
                 for (int i = 0; i < 8; ++i)
@@ -195,8 +214,8 @@ __global__ void __launch_bounds__(1024) add_rmsnorm_fp8_kernel(const T* __restri
         }
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-            const double d = r[j][i];
-            ss = fma(d, d, ss);
+            const double x = r[j][i];
+            ss = fma(x, x, ss);
         }
     }
 #pragma unroll
@@ -206,26 +225,48 @@ __global__ void __launch_bounds__(1024) add_rmsnorm_fp8_kernel(const T* __restri
     ss = 0.0;
     for (int w = 0; w < static_cast<int>(blockDim.x >> 5); ++w) ss += red[w];
     const double rs = 1.0 / sqrt(ss / k + kNormEps);
+    const float rs_f = static_cast<float>(rs);
+    const double rs448 = rs * (1.0 / static_cast<double>(kFp8Max));
     const int per_row = (k + kFp8Block - 1) / kFp8Block;
 #pragma unroll
     for (int j = 0; j < CHUNKS; ++j) {
         const int c = static_cast<int>(threadIdx.x + j * blockDim.x) * 8;
         const int live = max(0, min(8, k - c));
-        float w[8];
-        load8_ragged(gamma + (live ? c : 0), live, vec, w);
-        unsigned long long a = 0;
+        float w[8], p[8];
+        to_floats(load_raw8<VEC>(gamma + (live ? c : 0), live), w);
+        uint32_t a = 0;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) a = umax(a, abs_bits(static_cast<double>(r[j][i]) * static_cast<double>(w[i])));
+        for (int i = 0; i < 8; ++i) {
+            p[i] = r[j][i] * w[i];
+            a = umax(a, abs_bits(p[i]));
+        }
 #pragma unroll
         for (int o = kLanesPerGroup / 2; o; o >>= 1) a = umax(a, __shfl_xor_sync(0xffffffffu, a, o));
-        const double top = __longlong_as_double(static_cast<long long>(a)) * rs;
-        float s = static_cast<float>(top / static_cast<double>(kFp8Max));
+        float rest = -INFINITY;  // |r gamma| less its rounded value, at the largest
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            if (abs_bits(p[i]) == a) rest = fmaxf(rest, fmaf(fabsf(r[j][i]), fabsf(w[i]), -fabsf(p[i])));
+#pragma unroll
+        for (int o = kLanesPerGroup / 2; o; o >>= 1) rest = fmaxf(rest, __shfl_xor_sync(0xffffffffu, rest, o));
+        double top = static_cast<double>(__uint_as_float(a)) + static_cast<double>(rest);
+        // products that leave the range where they and their remainders are exact: 64 bits throughout
+        const bool far = !(__uint_as_float(a) < 1e30f) || (a != 0u && __uint_as_float(a) < 1e-20f);
+        if (__any_sync(0xffffffffu, far || (a == 0u))) {
+            unsigned long long e = 0;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) e = umax(e, abs_bits(static_cast<double>(r[j][i]) * static_cast<double>(w[i])));
+#pragma unroll
+            for (int o = kLanesPerGroup / 2; o; o >>= 1) e = umax(e, __shfl_xor_sync(0xffffffffu, e, o));
+            top = __longlong_as_double(static_cast<long long>(e));
+        }
+        float s = static_cast<float>(top * rs448);
         if (!(s <= 3.4e38f)) s = __uint_as_float(0x7fffffffu);
-        GroupScale g = group_scale(s);
-        const float f = s > 0.0f ? static_cast<float>(rs / static_cast<double>(s)) : 0.0f;
-        g.exact_only |= !(f < 1e30f) || !(f > 1e-30f && fabs(top) < 1e30);
+        GroupScale g;
+        g.s = s;
+        g.inv = s > 0.0f ? __fdividef(rs_f, s) : 0.0f;  // of the products, within 4 ulp
+        g.exact_only = far || (s > 0.0f && (s < 1e-30f || !(g.inv < 1e30f) || !(g.inv > 1e-30f)));
         const uint2 b = quantise8(
-            g, [&](int i) { return r[j][i] * w[i] * f; },
+            g, [&](int i) { return p[i] * g.inv; },
             [&](int i) { return static_cast<double>(r[j][i]) * static_cast<double>(w[i]) * rs; });
         if (live) {
             store_bytes(q + row * ldq + c, b, live);
@@ -234,38 +275,59 @@ __global__ void __launch_bounds__(1024) add_rmsnorm_fp8_kernel(const T* __restri
     }
 }
 
-template <typename T>
+template <typename T, bool VEC>
 cudaError_t launch_norm_typed(const void* delta, const void* residual, void* sum, const float* gamma, uint8_t* q,
-                              size_t ldq, float* scale, int n, int k, cudaStream_t s) {
-    const bool vec = (static_cast<size_t>(k) * sizeof(T)) % 16 == 0;
+                              size_t ldq, float* scale, int n, int k, int num_sms, cudaStream_t s) {
     const int chunks = (k + 7) / 8;
     const T *d = static_cast<const T*>(delta), *r = static_cast<const T*>(residual);
     T* o = static_cast<T*>(sum);
     count_launch();
     auto threads = [&](int per) { return ((chunks + per - 1) / per + 31) / 32 * 32; };
-    if (chunks <= 256) add_rmsnorm_fp8_kernel<T, 1><<<n, threads(1), 0, s>>>(d, r, o, gamma, q, ldq, scale, k, vec);
-    else if (chunks <= 1024) add_rmsnorm_fp8_kernel<T, 2><<<n, threads(2), 0, s>>>(d, r, o, gamma, q, ldq, scale, k, vec);
-    else add_rmsnorm_fp8_kernel<T, 4><<<n, threads(4), 0, s>>>(d, r, o, gamma, q, ldq, scale, k, vec);
+    // Few rows: as many threads as a row has chunks, for the shortest chain; many: more columns a thread, so that an
+    // SM holds more rows at different points of theirs.
+    const bool few = n <= 2 * num_sms;
+    if (chunks <= 256 && (few || chunks <= 64))
+        add_rmsnorm_fp8_kernel<T, 1, 256, VEC><<<n, threads(1), 0, s>>>(d, r, o, gamma, q, ldq, scale, k);
+    else if (chunks <= 512)
+        add_rmsnorm_fp8_kernel<T, 2, 256, VEC><<<n, threads(2), 0, s>>>(d, r, o, gamma, q, ldq, scale, k);
+    else if (chunks <= 1024)
+        add_rmsnorm_fp8_kernel<T, 4, 256, VEC><<<n, threads(4), 0, s>>>(d, r, o, gamma, q, ldq, scale, k);
+    else
+        add_rmsnorm_fp8_kernel<T, 4, 1024, VEC><<<n, threads(4), 0, s>>>(d, r, o, gamma, q, ldq, scale, k);
     return cudaGetLastError();
 }
 
-template <typename T>
-cudaError_t launch_quantize_typed(const void* xv, size_t ldx, uint8_t* q, size_t ldq, float* scale, int n, int k,
-                                  int rows, int num_sms, cudaStream_t s) {
-    const T* x = static_cast<const T*>(xv);
-    const bool vec = reinterpret_cast<uintptr_t>(x) % 16 == 0 && (ldx * sizeof(T)) % 16 == 0;
+template <typename T, bool VEC>
+cudaError_t launch_quantize_typed(const T* x, size_t ldx, uint8_t* q, size_t ldq, float* scale, int n, int k, int rows,
+                                  int num_sms, cudaStream_t s) {
     const uint32_t per_row = static_cast<uint32_t>((k - 1) / kFp8Block + 1);
     count_launch();
     if (rows == 1) {
         const uint32_t groups = static_cast<uint32_t>(n) * per_row;
         const uint32_t ctas = (groups + 15) / 16, most = static_cast<uint32_t>(num_sms) * 32;
-        quantize_rows_kernel<T><<<ctas < most ? ctas : most, 256, 0, s>>>(x, ldx, q, ldq, scale, groups,
-                                                                          FastDiv(per_row), k, vec);
+        quantize_rows_kernel<T, VEC><<<ctas < most ? ctas : most, 256, 0, s>>>(x, ldx, q, ldq, scale, groups,
+                                                                               FastDiv(per_row), k);
     } else {
         const uint32_t blocks = static_cast<uint32_t>((n - 1) / kFp8Block + 1) * per_row;
-        quantize_blocks_kernel<T><<<blocks, 256, 0, s>>>(x, ldx, q, ldq, scale, FastDiv(per_row), n, k, vec);
+        quantize_blocks_kernel<T, VEC><<<blocks, 256, 0, s>>>(x, ldx, q, ldq, scale, FastDiv(per_row), n, k);
     }
     return cudaGetLastError();
+}
+
+// Whole 16-byte loads: k in eights, rows that stay aligned.
+template <typename T>
+cudaError_t launch_quantize_typed(const void* xv, size_t ldx, uint8_t* q, size_t ldq, float* scale, int n, int k,
+                                  int rows, int num_sms, cudaStream_t s) {
+    const T* x = static_cast<const T*>(xv);
+    const bool vec = k % 8 == 0 && reinterpret_cast<uintptr_t>(x) % 16 == 0 && (ldx * sizeof(T)) % 16 == 0;
+    return vec ? launch_quantize_typed<T, true>(x, ldx, q, ldq, scale, n, k, rows, num_sms, s)
+               : launch_quantize_typed<T, false>(x, ldx, q, ldq, scale, n, k, rows, num_sms, s);
+}
+template <typename T>
+cudaError_t launch_norm_typed(const void* delta, const void* residual, void* sum, const float* gamma, uint8_t* q,
+                              size_t ldq, float* scale, int n, int k, int num_sms, cudaStream_t s) {
+    return k % 8 == 0 ? launch_norm_typed<T, true>(delta, residual, sum, gamma, q, ldq, scale, n, k, num_sms, s)
+                      : launch_norm_typed<T, false>(delta, residual, sum, gamma, q, ldq, scale, n, k, num_sms, s);
 }
 
 }  // namespace
@@ -281,11 +343,11 @@ cudaError_t launch_quantize_fp8(int dtype, const void* x, size_t ldx, uint8_t* q
 }
 
 cudaError_t launch_add_rmsnorm_fp8(int dtype, const void* delta, const void* residual, void* sum, const float* gamma,
-                                   uint8_t* q, size_t ldq, float* scale, int n, int k, cudaStream_t s) {
+                                   uint8_t* q, size_t ldq, float* scale, int n, int k, int num_sms, cudaStream_t s) {
     switch (dtype) {
-        case kF32: return launch_norm_typed<float>(delta, residual, sum, gamma, q, ldq, scale, n, k, s);
-        case kBF16: return launch_norm_typed<__nv_bfloat16>(delta, residual, sum, gamma, q, ldq, scale, n, k, s);
-        case kF16: return launch_norm_typed<__half>(delta, residual, sum, gamma, q, ldq, scale, n, k, s);
+        case kF32: return launch_norm_typed<float>(delta, residual, sum, gamma, q, ldq, scale, n, k, num_sms, s);
+        case kBF16: return launch_norm_typed<__nv_bfloat16>(delta, residual, sum, gamma, q, ldq, scale, n, k, num_sms, s);
+        case kF16: return launch_norm_typed<__half>(delta, residual, sum, gamma, q, ldq, scale, n, k, num_sms, s);
         default: return cudaErrorInvalidValue;
     }
 }

@@ -399,7 +399,7 @@ cudaError_t launch_quantize_fp8(int dtype, const void* x, size_t ldx, uint8_t* q
 // sum = residual + delta (delta may be null: then sum is not written), q and scale of its RMSNorm.
 constexpr int kNormMaxK = 32768;  // a row is kept in one CTA's registers
 cudaError_t launch_add_rmsnorm_fp8(int dtype, const void* delta, const void* residual, void* sum, const float* gamma,
-                                   uint8_t* q, size_t ldq, float* scale, int n, int k, cudaStream_t s);
+                                   uint8_t* q, size_t ldq, float* scale, int n, int k, int num_sms, cudaStream_t s);
 // y (+)= xq . wq^T with the scales, mode as GemvMode (Plain / SwiGLU / Residual).
 cudaError_t launch_linear_fp8(int mode, int dtype, const uint8_t* xq, size_t ldx, const float* xs, const uint8_t* wq,
                               size_t ldw, const float* ws, const float* bias, void* y, int n, int m, int k, int num_sms,
