@@ -359,8 +359,8 @@ XL_API int xl_op_attn_prefill(float* qkv, const float* rope, float* kc, float* v
  *
  * Common to them: matrices are row-major; `dtype` is the element type of the
  * rows (XL_F32, XL_BF16, XL_F16); device pointers belong to the current
- * device, the stream too (a pointer of another device, or of the host, is
- * refused with XL_ERR_ARG); matrix and row pointers are 16-byte aligned, every
+ * device, the stream too (a pointer of another device, or to pageable host
+ * memory, is refused with XL_ERR_ARG); matrix and row pointers are 16-byte aligned, every
  * other pointer aligned to its element, NULL only where said; each call is one
  * kernel, asynchronous on `stream`, allocates nothing, and may be captured
  * into a graph.  Inputs and outputs do not overlap except where said.

@@ -1,6 +1,8 @@
 // extern "C" surface of libxl_engine.so (declared in include/xl_engine.h).
+#include <cuda.h>
 #include <nccl.h>
 
+#include <atomic>
 #include <cstring>
 #include <initializer_list>
 #include <string>
@@ -469,27 +471,46 @@ bool aligned(const void* p, size_t to) { return reinterpret_cast<uintptr_t>(p) %
 size_t type_bytes(int dtype) { return dtype == xl::kF32 ? 4 : 2; }
 bool type_ok(int dtype) { return dtype == xl::kF32 || dtype == xl::kBF16 || dtype == xl::kF16; }
 
-// Each pointer (null ones aside) has to be memory of the current device, whose
-// SM count goes to *sms: a kernel given another device's or the host's memory
-// would fault.
+// Each pointer (null ones aside) has to be memory that the current device
+// owns, whose SM count goes to *sms: a kernel given another device's or
+// pageable host memory would fault.  One attribute of the driver's a pointer
+// (about 0.1 us; the runtime's call collects several).
+using PointerAttributeFn = CUresult (*)(void*, CUpointer_attribute, CUdeviceptr);
+PointerAttributeFn pointer_attribute() {
+    static const PointerAttributeFn fn = [] {
+        void* p = nullptr;
+        cudaDriverEntryPointQueryResult q;
+        const cudaError_t e = cudaGetDriverEntryPoint("cuPointerGetAttribute", &p, cudaEnableDefault, &q);
+        return e == cudaSuccess && q == cudaDriverEntryPointSuccess ? reinterpret_cast<PointerAttributeFn>(p) : nullptr;
+    }();
+    return fn;
+}
+
 int on_current_device(const char* what, std::initializer_list<const void*> ptrs, int* sms) {
+    constexpr int kDevices = 64;
+    static std::atomic<int> sm_count[kDevices];  // 0: not asked yet
     int dev = 0;
     int rc = cuda_status(cudaGetDevice(&dev), what);
     if (rc != XL_OK) return rc;
+    const PointerAttributeFn attribute = pointer_attribute();
+    if (!attribute) return cuda_status(cudaErrorNotSupported, what);
     for (const void* p : ptrs) {
         if (!p) continue;
-        cudaPointerAttributes a{};
-        const cudaError_t e = cudaPointerGetAttributes(&a, p);
-        if (e != cudaSuccess) {
-            cudaGetLastError();
-            return cuda_status(e, what);
-        }
-        if (a.type != cudaMemoryTypeManaged && (a.type != cudaMemoryTypeDevice || a.device != dev)) {
+        int owner = -1;
+        if (attribute(&owner, CU_POINTER_ATTRIBUTE_DEVICE_ORDINAL, reinterpret_cast<CUdeviceptr>(p)) != CUDA_SUCCESS ||
+            owner != dev) {
             xl::set_error(std::string(what) + ": a pointer is not memory of the current device");
             return XL_ERR_ARG;
         }
     }
-    return cuda_status(cudaDeviceGetAttribute(sms, cudaDevAttrMultiProcessorCount, dev), what);
+    const int known = dev < kDevices ? sm_count[dev].load(std::memory_order_relaxed) : 0;
+    if (known) {
+        *sms = known;
+        return XL_OK;
+    }
+    rc = cuda_status(cudaDeviceGetAttribute(sms, cudaDevAttrMultiProcessorCount, dev), what);
+    if (rc == XL_OK && dev < kDevices) sm_count[dev].store(*sms, std::memory_order_relaxed);
+    return rc;
 }
 
 // Null if the cache's description is in order, else what is wrong with it.

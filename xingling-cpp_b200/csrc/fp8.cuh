@@ -97,16 +97,19 @@ __device__ __forceinline__ uint32_t e4m3_of(double v) {
     return e4m3x2(f, 0.0f) & 0xffu;
 }
 
-// Whether a 32-bit quotient that is at most 8 units in the last place off may
-// lie on the other side of a border between two e4m3 values than the exact
-// one does.  From 2^-6 on borders are where the 4th bit after the leading one
-// is set and nothing follows; below (steps of 2^-9) the odd multiples of 2^-10.
-__device__ __forceinline__ bool near_border_normal(float q) {
-    return ((__float_as_uint(q) - 0x7fff8u) & 0xfffffu) <= 16u;
-}
+// Quotients of the fast path are off by less than kQuotientError of
+// themselves and then raised by it, so they lie 0 to 16 units in the last
+// place above the exact ones: a quotient on the other side of a border between
+// two e4m3 values than the exact one, or on a border, is one of the 16 floats
+// from the border on.  From 2^-6 on borders are where the 4th bit after the
+// leading one is set and nothing follows: bits 4 .. 19 are those of 0x80000,
+// and this is 0.
+constexpr float kQuotientError = 4.76837158203125e-7f;  // 2^-21
+__device__ __forceinline__ uint32_t border_bits(float q) { return (__float_as_uint(q) & 0xffff0u) ^ 0x80000u; }
+// Below 2^-6 (steps of 2^-9) they are the odd multiples of 2^-10.
 __device__ __forceinline__ bool near_border_small(float q) {
     const float m = fabsf(q) * 1024.0f, r = rintf(m);
-    return m <= 16.0f && fabsf(m - r) < 1e-5f && (static_cast<int>(r) & 1);
+    return m <= 16.5f && fabsf(m - r) < 4e-5f && (static_cast<int>(r) & 1);
 }
 
 // n / d for 0 <= n < 2^31 with a multiplication (Granlund and Montgomery,

@@ -28,6 +28,7 @@
 #include <cuda_fp16.h>
 
 #include <algorithm>
+#include <atomic>
 
 #include "fp8.cuh"
 #include "tcgen05.cuh"
@@ -523,8 +524,16 @@ cudaError_t launch_tiled(const CUtensorMap& mx, const CUtensorMap& mw, const Lin
         }();
         if (!fits) return cudaErrorInvalidConfiguration;
     }
-    cudaError_t e = cudaFuncSetAttribute(linear_fp8_kernel<CG, T>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemLimit);
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
     if (e != cudaSuccess) return e;
+    static std::atomic<unsigned long long> allowed{0};  // devices on which the kernel may have this much shared memory
+    const unsigned long long bit = dev < 64 ? 1ull << dev : 0ull;
+    if (!(allowed.load(std::memory_order_relaxed) & bit)) {
+        e = cudaFuncSetAttribute(linear_fp8_kernel<CG, T>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemLimit);
+        if (e != cudaSuccess) return e;
+        allowed.fetch_or(bit, std::memory_order_relaxed);
+    }
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3(static_cast<unsigned>(grid));
     cfg.blockDim = dim3(TL::kThreads);

@@ -25,7 +25,7 @@ namespace {
 constexpr int kLanesPerGroup = 16;  // lanes that share a group: 8 columns each
 constexpr double kNormEps = 1e-6;   // as the engine's RMSNorm
 
-// What divides a group's values: the stored scale and its reciprocal.
+// What divides a group's values: the stored scale and its reciprocal (raised, see kQuotientError).
 struct GroupScale {
     float s, inv;
     bool exact_only;  // the reciprocal overflows (a scale near the smallest floats)
@@ -34,7 +34,7 @@ __device__ __forceinline__ GroupScale group_scale(float s) {
     GroupScale g;
     g.s = s;
     g.exact_only = s > 0.0f && s < 1e-30f;
-    g.inv = s > 0.0f ? __fdividef(1.0f, s) : 0.0f;  // within 2 ulp: s is below 2^126
+    g.inv = s > 0.0f ? __fdividef(1.0f + kQuotientError, s) : 0.0f;  // within 2 ulp: s is below 2^126
     return g;
 }
 
@@ -42,13 +42,14 @@ __device__ __forceinline__ GroupScale group_scale(float s) {
 template <typename Fast, typename Exact>
 __device__ __forceinline__ uint2 quantise8(const GroupScale& g, Fast fast, Exact y) {
     float q[8], least = INFINITY;
-    bool close = g.exact_only;
+    uint32_t bits = 1u;
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
         q[i] = fast(i);
-        close |= near_border_normal(q[i]);
+        bits = min(bits, border_bits(q[i]));
         least = fminf(least, fabsf(q[i]));
     }
+    bool close = g.exact_only || bits == 0u;
     if (least < 0.015625f) {
 #pragma unroll
         for (int i = 0; i < 8; ++i) close |= near_border_small(q[i]);
@@ -167,13 +168,21 @@ __global__ void __launch_bounds__(256) quantize_blocks_kernel(const T* __restric
     if (threadIdx.x == 0) scale[blockIdx.x] = g.s;
 }
 
+// 1 / sqrt(v) in 64 bits: Newton's iteration y (3 - v y^2) / 2 from the 32-bit
+// function, whose 2^-22 two steps square down below 2^-80.
+__device__ __forceinline__ double inverse_root(double v) {
+    if (!(v < 1e37)) return 1.0 / sqrt(v);
+    double y = rsqrtf(static_cast<float>(v));
+    y *= fma(-0.5 * v * y, y, 1.5);
+    return y * fma(-0.5 * v * y, y, 1.5);
+}
+
 // r = fl_T(residual + delta) (stored where there is a delta), rs =
 // 1 / sqrt(mean(r^2) + eps), y = r gamma rs, e4m3 per row and 128 columns.
 // One row a CTA, kept in registers (CHUNKS x 8 columns a thread), so each
 // input is read once.  The sum of squares is 64-bit and the largest |r gamma|
-// of a group is found exactly: as the largest fp32 product (rounding keeps the
-// order) and, among those that round to it, the largest remainder.  So a
-// group's scale and bytes do not depend on the order of the sum.
+// of a group is taken with the remainder of its fp32 product (rounding keeps
+// the order), so that a group's scale is the rounded exact one.
 template <typename T, int CHUNKS, int THREADS, bool VEC>
 __global__ void __launch_bounds__(THREADS) add_rmsnorm_fp8_kernel(const T* __restrict__ delta, const T* residual, T* sum,
                                                                   const float* __restrict__ gamma,
@@ -182,6 +191,7 @@ __global__ void __launch_bounds__(THREADS) add_rmsnorm_fp8_kernel(const T* __res
     __shared__ double red[32];
     const size_t row = blockIdx.x;
     const int warp = threadIdx.x >> 5;
+    const double per_k = 1.0 / k;
     Raw8<T> raw_r[CHUNKS], raw_d[CHUNKS];
 #pragma unroll
     for (int j = 0; j < CHUNKS; ++j) {
@@ -224,9 +234,9 @@ __global__ void __launch_bounds__(THREADS) add_rmsnorm_fp8_kernel(const T* __res
     __syncthreads();
     ss = 0.0;
     for (int w = 0; w < static_cast<int>(blockDim.x >> 5); ++w) ss += red[w];
-    const double rs = 1.0 / sqrt(ss / k + kNormEps);
-    const float rs_f = static_cast<float>(rs);
+    const double rs = inverse_root(fma(ss, per_k, kNormEps));
     const double rs448 = rs * (1.0 / static_cast<double>(kFp8Max));
+    const float rs_hi = static_cast<float>(rs448), rs_lo = static_cast<float>(rs448 - static_cast<double>(rs_hi));
     const int per_row = (k + kFp8Block - 1) / kFp8Block;
 #pragma unroll
     for (int j = 0; j < CHUNKS; ++j) {
@@ -234,37 +244,42 @@ __global__ void __launch_bounds__(THREADS) add_rmsnorm_fp8_kernel(const T* __res
         const int live = max(0, min(8, k - c));
         float w[8], p[8];
         to_floats(load_raw8<VEC>(gamma + (live ? c : 0), live), w);
-        uint32_t a = 0;
+        float own = -1.0f, own_r = 0.0f, own_w = 0.0f;  // the lane's largest product and its factors
+        bool nan = false;
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
             p[i] = r[j][i] * w[i];
-            a = umax(a, abs_bits(p[i]));
+            nan |= p[i] != p[i];
+            if (fabsf(p[i]) > own) own = fabsf(p[i]), own_r = r[j][i], own_w = w[i];
         }
+        const uint32_t mine = nan ? 0x7fffffffu : __float_as_uint(own);
+        uint32_t a = mine;
 #pragma unroll
         for (int o = kLanesPerGroup / 2; o; o >>= 1) a = umax(a, __shfl_xor_sync(0xffffffffu, a, o));
-        float rest = -INFINITY;  // |r gamma| less its rounded value, at the largest
-#pragma unroll
-        for (int i = 0; i < 8; ++i)
-            if (abs_bits(p[i]) == a) rest = fmaxf(rest, fmaf(fabsf(r[j][i]), fabsf(w[i]), -fabsf(p[i])));
-#pragma unroll
-        for (int o = kLanesPerGroup / 2; o; o >>= 1) rest = fmaxf(rest, __shfl_xor_sync(0xffffffffu, rest, o));
-        double top = static_cast<double>(__uint_as_float(a)) + static_cast<double>(rest);
-        // products that leave the range where they and their remainders are exact: 64 bits throughout
-        const bool far = !(__uint_as_float(a) < 1e30f) || (a != 0u && __uint_as_float(a) < 1e-20f);
-        if (__any_sync(0xffffffffu, far || (a == 0u))) {
+        // the group's largest product, exactly: its rounded value and the remainder
+        const uint32_t holders = __ballot_sync(0xffffffffu, mine == a) & (0xffffu << (threadIdx.x & 16));
+        const int holder = __ffs(holders) - 1;
+        const float wr = __shfl_sync(0xffffffffu, own_r, holder), ww = __shfl_sync(0xffffffffu, own_w, holder);
+        const float top = __uint_as_float(a), rest = fmaf(fabsf(wr), fabsf(ww), -top);
+        // top / 448 / root to 2^-46, then rounded once
+        const float t = top * rs_hi;
+        float s = t + (fmaf(top, rs_hi, -t) + fmaf(top, rs_lo, rest * rs_hi));
+        // out of the range where these are exact (and for a group of zeros, where nothing is lost): 64 bits
+        const bool far = !(top < 1e30f) || top < 1e-20f || !(rs_hi > 1e-15f);
+        if (__any_sync(0xffffffffu, far)) {
             unsigned long long e = 0;
 #pragma unroll
             for (int i = 0; i < 8; ++i) e = umax(e, abs_bits(static_cast<double>(r[j][i]) * static_cast<double>(w[i])));
 #pragma unroll
             for (int o = kLanesPerGroup / 2; o; o >>= 1) e = umax(e, __shfl_xor_sync(0xffffffffu, e, o));
-            top = __longlong_as_double(static_cast<long long>(e));
+            if (far) s = static_cast<float>(__longlong_as_double(static_cast<long long>(e)) * rs448);
         }
-        float s = static_cast<float>(top * rs448);
         if (!(s <= 3.4e38f)) s = __uint_as_float(0x7fffffffu);
         GroupScale g;
         g.s = s;
-        g.inv = s > 0.0f ? __fdividef(rs_f, s) : 0.0f;  // of the products, within 4 ulp
-        g.exact_only = far || (s > 0.0f && (s < 1e-30f || !(g.inv < 1e30f) || !(g.inv > 1e-30f)));
+        // 448 (1 + error) / top, within 4 ulp of rs / s: the products are at most top
+        g.inv = s > 0.0f ? __fdividef(rs_hi * (kFp8Max * (1.0f + kQuotientError)), s) : 0.0f;
+        g.exact_only = far;
         const uint2 b = quantise8(
             g, [&](int i) { return p[i] * g.inv; },
             [&](int i) { return static_cast<double>(r[j][i]) * static_cast<double>(w[i]) * rs; });
