@@ -511,10 +511,39 @@ __global__ void __launch_bounds__(Tile<CG>::kThreads, 1)
     }
 }
 
+using LinearKernel = void (*)(CUtensorMap, CUtensorMap, LinearParams);
+
+// `allowed`: the devices on which the kernel may already have this much shared memory.
+cudaError_t launch_linear(LinearKernel kernel, std::atomic<unsigned long long>& allowed, const CUtensorMap& mx,
+                          const CUtensorMap& mw, const LinearParams& p, int grid, int threads, int cluster, int smem,
+                          cudaStream_t s) {
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return e;
+    const unsigned long long bit = dev < 64 ? 1ull << dev : 0ull;
+    if (!(allowed.load(std::memory_order_relaxed) & bit)) {
+        e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemLimit);
+        if (e != cudaSuccess) return e;
+        allowed.fetch_or(bit, std::memory_order_relaxed);
+    }
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(static_cast<unsigned>(grid));
+    cfg.blockDim = dim3(static_cast<unsigned>(threads));
+    cfg.dynamicSmemBytes = static_cast<size_t>(smem);
+    cfg.stream = s;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = static_cast<unsigned>(cluster);
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = cluster > 1 ? 1 : 0;
+    count_launch();
+    return cudaLaunchKernelEx(&cfg, kernel, mx, mw, p);
+}
+
 template <int CG, typename T>
 cudaError_t launch_tiled(const CUtensorMap& mx, const CUtensorMap& mw, const LinearParams& p, int grid, cudaStream_t s) {
     using TL = Tile<CG>;
-    const int smem = p.stages * p.stage_bytes + TL::kStoreBytes + kBarBytes + 1024;
     if (CG == 2) {
         // the warpgroups' register shares have to fit what the CTA launches with, or the larger one never comes
         static const bool fits = [] {
@@ -524,33 +553,280 @@ cudaError_t launch_tiled(const CUtensorMap& mx, const CUtensorMap& mw, const Lin
         }();
         if (!fits) return cudaErrorInvalidConfiguration;
     }
-    int dev = 0;
-    cudaError_t e = cudaGetDevice(&dev);
-    if (e != cudaSuccess) return e;
-    static std::atomic<unsigned long long> allowed{0};  // devices on which the kernel may have this much shared memory
-    const unsigned long long bit = dev < 64 ? 1ull << dev : 0ull;
-    if (!(allowed.load(std::memory_order_relaxed) & bit)) {
-        e = cudaFuncSetAttribute(linear_fp8_kernel<CG, T>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemLimit);
-        if (e != cudaSuccess) return e;
-        allowed.fetch_or(bit, std::memory_order_relaxed);
-    }
-    cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3(static_cast<unsigned>(grid));
-    cfg.blockDim = dim3(TL::kThreads);
-    cfg.dynamicSmemBytes = static_cast<size_t>(smem);
-    cfg.stream = s;
-    cudaLaunchAttribute attr[1];
-    const int cluster = CG == 2 ? 2 : p.split;
-    attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = static_cast<unsigned>(cluster);
-    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = cluster > 1 ? 1 : 0;
-    count_launch();
-    return cudaLaunchKernelEx(&cfg, linear_fp8_kernel<CG, T>, mx, mw, p);
+    static std::atomic<unsigned long long> allowed{0};
+    return launch_linear(linear_fp8_kernel<CG, T>, allowed, mx, mw, p, grid, TL::kThreads, CG == 2 ? 2 : p.split,
+                         p.stages * p.stage_bytes + TL::kStoreBytes + kBarBytes + 1024, s);
 }
 
-// ---- few tokens: the weights stream through registers ----
+// ---- up to 64 tokens: features on the TMEM lanes ----
+//
+// The operands change places: 128 features are the MMA's M, the tokens its N
+// (16, 32 or 64).  A K-block then leaves few columns to drain, a lane's
+// results of one token lie next to its neighbours' in y, and the tensor core
+// takes a K-block in the time its weights take to arrive.  Fewer tiles than
+// SMs split K over the CTAs of a cluster, whose partial tiles meet in
+// distributed shared memory.
+
+template <int N>
+struct Few {
+    static constexpr int kAccs = N == 64 ? 4 : 8;
+    static constexpr int kColumns = kAccs * N;
+    static constexpr int kThreads = 192;
+    static constexpr int kStage = kOpBytes + N * kFp8Block;
+    static constexpr int kScaleBytes = 4 * N * 4;  // a warp's N scales
+    static constexpr uint32_t kIdesc = (1u << 4) | (static_cast<uint32_t>(N >> 3) << 17) | (static_cast<uint32_t>(128 >> 4) << 24);
+};
+
+// N TMEM columns of the warp's 32 lanes, 16 at a time.
+__device__ __forceinline__ void tmem_load16(uint32_t addr, uint32_t* r) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, "
+        "[%16];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+          "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+        : "r"(addr));
+}
+__device__ __forceinline__ void tmem_wait16(uint32_t* r) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+                 : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]),
+                   "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15])
+                 :
+                 : "memory");
+}
+
+template <int N, typename T>
+__global__ void __launch_bounds__(Few<N>::kThreads, 2)
+    linear_fp8_few_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_w,
+                          const LinearParams p) {
+    using F = Few<N>;
+    extern __shared__ __align__(1024) char smem_raw[];
+    char* ring = reinterpret_cast<char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
+    float* scales = reinterpret_cast<float*>(ring + p.stages * F::kStage);
+    uint64_t* full = reinterpret_cast<uint64_t*>(reinterpret_cast<char*>(scales) + F::kScaleBytes);
+    uint64_t* empty = full + kMaxStages;
+    uint64_t* done = empty + kMaxStages;
+    uint64_t* freed = done + F::kAccs;
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(freed + F::kAccs);
+
+    const int warp = __shfl_sync(0xffffffffu, static_cast<int>(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
+    const uint32_t rank = p.split > 1 ? cluster_rank() : 0u;
+    const int unit = static_cast<int>(blockIdx.x) / p.split, units = static_cast<int>(gridDim.x) / p.split;
+    const int kb0 = static_cast<int>(static_cast<long long>(rank) * p.blocks / p.split);
+    const int kb1 = static_cast<int>(static_cast<long long>(rank + 1) * p.blocks / p.split);
+
+    if (warp == 0) {
+        if (elect_one()) asm volatile("prefetch.tensormap [%0];\n\tprefetch.tensormap [%1];" ::"l"(&map_x), "l"(&map_w) : "memory");
+        if (lane < p.stages) {
+            mbar_init(&full[lane], 1);
+            mbar_init(&empty[lane], 1);
+        }
+        if (lane < F::kAccs) {
+            mbar_init(&done[lane], 1);
+            mbar_init(&freed[lane], 4);
+        }
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 1) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)),
+                     "n"(F::kColumns)
+                     : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    __syncthreads();
+    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    const uint32_t tmem = *tmem_slot;
+
+    if (warp == 0) {
+        int s = 0;
+        uint32_t ph = 0, issued = 0;
+        bool ok = true;
+        for (int t = unit; t < p.tiles_m && ok; t += units) {
+            for (int kb = kb0; kb < kb1; ++kb) {
+                if (!wait_warp(&empty[s], ph ^ 1u)) {
+                    ok = false;
+                    break;
+                }
+                const uint32_t st = smem_u32(ring + s * F::kStage);
+                if (elect_one()) {
+                    mbar_expect_tx(&full[s], F::kStage);
+                    load_tile<1>(st, &map_w, kb * kFp8Block, t * 128, smem_u32(&full[s]));
+                    load_tile<1>(st + kOpBytes, &map_x, kb * kFp8Block, 0, smem_u32(&full[s]));
+                }
+                __syncwarp();
+                ++issued;
+                if (++s == p.stages) s = 0, ph ^= 1u;
+            }
+        }
+        if (!ok) {
+            // the copies in flight land before the CTA leaves
+            for (uint32_t i = 0; i < min(issued, static_cast<uint32_t>(p.stages)); ++i) {
+                if (s == 0) s = p.stages, ph ^= 1u;
+                --s;
+                wait_warp(&full[s], ph);
+            }
+        }
+    } else if (warp == 1) {
+        int s = 0, a = 0;
+        uint32_t ph = 0, pa = 0;
+        bool ok = true;
+        for (int t = unit; t < p.tiles_m && ok; t += units) {
+            for (int kb = kb0; kb < kb1; ++kb) {
+                if (!wait_warp(&freed[a], pa ^ 1u) || !wait_warp(&full[s], ph)) {
+                    ok = false;
+                    break;
+                }
+                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                const uint32_t st = smem_u32(ring + s * F::kStage);
+                const uint64_t dw = umma_desc(st), dx = umma_desc(st + kOpBytes);
+                const uint32_t acc = tmem + static_cast<uint32_t>(a * N);
+                if (elect_one()) {
+#pragma unroll
+                    for (int ks = 0; ks < 4; ++ks) mma_e4m3<1>(acc, dw + 2 * ks, dx + 2 * ks, F::kIdesc, ks != 0);
+                    commit<1>(&empty[s]);
+                    commit<1>(&done[a]);
+                }
+                __syncwarp();
+                if (++s == p.stages) s = 0, ph ^= 1u;
+                if (++a == F::kAccs) a = 0, pa ^= 1u;
+            }
+        }
+    } else {
+        const int q = warp & 3;
+        float* sc = scales + (warp - 2) * N;
+        int a = 0;
+        uint32_t pa = 0;
+        bool ok = true;
+        const float* xs[N / 32 + 1];
+#pragma unroll
+        for (int i = 0; i < (N + 31) / 32; ++i) xs[i] = p.xs + static_cast<size_t>(min(32 * i + lane, p.n - 1)) * p.blocks;
+        for (int t = unit; t < p.tiles_m; t += units) {
+            const float* ws = p.ws + static_cast<size_t>(t) * p.blocks;
+            const int j = t * 128 + 32 * q + lane;
+            const float bias = p.bias && j < p.m ? p.bias[j] : 0.0f;
+            unsigned long long acc[N / 2];
+#pragma unroll
+            for (int i = 0; i < N / 2; ++i) acc[i] = 0;
+            float sx[(N + 31) / 32], sw = ws[kb0];
+#pragma unroll
+            for (int i = 0; i < (N + 31) / 32; ++i) sx[i] = xs[i][kb0];
+            bool ready = mbar_try_wait(&done[a], pa);
+#pragma unroll 1
+            for (int kb = kb0; kb < kb1; ++kb) {
+#pragma unroll
+                for (int i = 0; i < (N + 31) / 32; ++i)
+                    if (32 * i + lane < N) sc[32 * i + lane] = sx[i] * sw;
+                const int next = min(kb + 1, kb1 - 1);
+                sw = ws[next];
+#pragma unroll
+                for (int i = 0; i < (N + 31) / 32; ++i) sx[i] = xs[i][next];
+                __syncwarp();
+                if (ok && !__all_sync(0xffffffffu, ready)) ok = wait_warp(&done[a], pa);
+                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                uint32_t r[N];
+                const uint32_t ta = tmem + (static_cast<uint32_t>(32 * q) << 16) + static_cast<uint32_t>(a * N);
+                if (ok) {
+#pragma unroll
+                    for (int i = 0; i < N; i += 16) tmem_load16(ta + i, r + i);
+#pragma unroll
+                    for (int i = 0; i < N; i += 16) tmem_wait16(r + i);
+                }
+                asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+                __syncwarp();
+                if (elect_one())
+                    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(&freed[a])) : "memory");
+                if (++a == F::kAccs) a = 0, pa ^= 1u;
+                if (kb + 1 < kb1) ready = mbar_try_wait(&done[a], pa);
+                if (ok) {
+#pragma unroll
+                    for (int i = 0; i < N / 4; ++i) {
+                        const ulonglong2 s4 = reinterpret_cast<const ulonglong2*>(sc)[i];
+                        fma2(acc[2 * i], pack2(r[4 * i], r[4 * i + 1]), s4.x);
+                        fma2(acc[2 * i + 1], pack2(r[4 * i + 2], r[4 * i + 3]), s4.y);
+                    }
+                }
+                __syncwarp();
+            }
+            if (!ok) {  // a wait ran out: the results say so
+#pragma unroll
+                for (int i = 0; i < N / 2; ++i) acc[i] = 0x7fffffff7fffffffull;
+            }
+            if (p.split == 1) {
+                T* y = static_cast<T*>(p.y);
+                const bool swiglu = p.mode == kGemvSwiGLU;
+#pragma unroll
+                for (int i = 0; i < N; ++i) {
+                    if (i >= p.n) break;
+                    const float2 v2 = unpack2(acc[i / 2]);
+                    const float v = (i & 1 ? v2.y : v2.x) + bias;
+                    if (swiglu) {
+                        const float c = __shfl_xor_sync(0xffffffffu, v, 1);
+                        if (!(lane & 1) && j < p.m) y[static_cast<size_t>(i) * (p.m >> 1) + (j >> 1)] = from_float<T>(silu_fast(v) * c);
+                    } else if (j < p.m) {
+                        put(y + static_cast<size_t>(i) * p.m + j, v, p.mode);
+                    }
+                }
+            } else {
+                // every K-block of this CTA has been multiplied: the ring is free for the partial tile [tokens][128]
+                float* part = reinterpret_cast<float*>(ring);
+#pragma unroll
+                for (int i = 0; i < N; ++i) {
+                    const float2 v2 = unpack2(acc[i / 2]);
+                    if (i < p.n) part[i * 128 + 32 * q + lane] = i & 1 ? v2.y : v2.x;
+                }
+            }
+        }
+        asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    }
+    if (p.split > 1) {
+        __syncwarp();
+        cluster_sync();
+        // A cluster has one tile; this CTA finishes its share of the (token, 4 features) pieces.
+        const uint32_t part = smem_u32(ring);
+        const int pieces = p.n * 32, e1 = static_cast<int>(static_cast<long long>(rank + 1) * pieces / p.split);
+        T* y = static_cast<T*>(p.y);
+        for (int e = static_cast<int>(static_cast<long long>(rank) * pieces / p.split) + threadIdx.x; e < e1; e += F::kThreads) {
+            const int tok = e >> 5, j = unit * 128 + (e & 31) * 4;
+            float4 v[kMaxSplit];
+#pragma unroll
+            for (int k = 0; k < kMaxSplit; ++k) {
+                v[k] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                if (k < p.split)
+                    asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+                                 : "=f"(v[k].x), "=f"(v[k].y), "=f"(v[k].z), "=f"(v[k].w)
+                                 : "r"(cluster_addr(part + static_cast<uint32_t>(e) * 16, k))
+                                 : "memory");
+            }
+            float o[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+            for (int i = 0; i < 4; ++i) o[i] = p.bias && j + i < p.m ? p.bias[j + i] : 0.0f;
+            float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+            for (int k = 0; k < kMaxSplit; ++k) sum[0] += v[k].x, sum[1] += v[k].y, sum[2] += v[k].z, sum[3] += v[k].w;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) o[i] += sum[i];
+            if (p.mode == kGemvSwiGLU) {
+                T* dst = y + static_cast<size_t>(tok) * (p.m >> 1) + (j >> 1);
+                if (j < p.m) dst[0] = from_float<T>(silu_fast(o[0]) * o[1]);
+                if (j + 2 < p.m) dst[1] = from_float<T>(silu_fast(o[2]) * o[3]);
+            } else {
+                T* dst = y + static_cast<size_t>(tok) * p.m + j;
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    if (j + i < p.m) put(dst + i, o[i], p.mode);
+            }
+        }
+    }
+    __syncwarp();
+    __syncthreads();
+    if (p.split > 1) cluster_sync();  // no CTA leaves while another may read its shared memory
+    if (warp == 1) {
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "n"(F::kColumns) : "memory");
+    }
+}
+
+// ---- few tokens and weights: the weights stream through registers ----
 
 // 16 bytes of a row from column c on, zeros past k (the bytes between k and the row's pitch are not touched).
 __device__ __forceinline__ uint4 load_row16(const uint8_t* row, int c, int k) {
@@ -570,14 +846,13 @@ __device__ __forceinline__ void mma_16x8x32(float (&d)[4], uint32_t a0, uint32_t
         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
-// One K-block's operands of a lane: weight rows g and g + 8, NT token tiles, 2
-// x 16 bytes each.  A lane reads 16 consecutive bytes where the MMA's layout
-// wants 4 x 4: the columns are permuted alike in both operands, so the sums
-// are the same.
-template <int NT>
+// One K-block's operands of a lane: weight rows g and g + 8 and the token's
+// row, 2 x 16 bytes each.  A lane reads 16 consecutive bytes where the MMA's
+// layout wants 4 x 4: the columns are permuted alike in both operands, so the
+// sums are the same.
 struct StreamBlock {
-    uint4 a[2][2], b[NT][2];
-    float s[NT][2];
+    uint4 a[2][2], b[2];
+    float s[2];
 };
 
 struct StreamParams {
@@ -588,77 +863,66 @@ struct StreamParams {
     int mode, n, m, k, blocks;
 };
 
+constexpr int kStreamTokens = 8;            // columns of the MMA
+constexpr long long kStreamBytes = 9 << 20;  // most weights: beyond, TMA and tcgen05 take less (see launch_tokens)
+constexpr int kStreamDepth = 4;             // K-blocks of a warp in flight
+constexpr int kStreamWarps = 16;            // most
+
 // 16 weight rows a CTA, its warps share the K-blocks and add up through shared
-// memory.  No TMEM, no barriers but one: a decode step's product is a stream
-// of weights, and every load of a CTA is in flight at once.
-template <int NT, int DEPTH, typename T>
-__global__ void __launch_bounds__(512) linear_fp8_stream_kernel(const StreamParams p) {
-    extern __shared__ float part[];  // [warps][16][NT * 8 + 1]
-    constexpr int kPitch = NT * 8 + 1;
+// memory.  No TMEM, no barriers but one: the product of a small decode step is
+// one memory round trip, and every load of a CTA is in flight at once.
+template <typename T>
+__global__ void __launch_bounds__(32 * kStreamWarps) linear_fp8_stream_kernel(const StreamParams p) {
+    constexpr int kPitch = kStreamTokens + 1;
+    __shared__ float part[kStreamWarps * 16 * kPitch];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = static_cast<int>(blockDim.x >> 5);
     const int g = lane >> 2, t = lane & 3, row0 = static_cast<int>(blockIdx.x) * 16;
     const uint8_t* wr[2];
-    const uint8_t* xr[NT];
-    const float* sx[NT][2];
+    const float* sx[2];
 #pragma unroll
-    for (int i = 0; i < 2; ++i) wr[i] = p.wq + static_cast<size_t>(min(row0 + g + 8 * i, p.m - 1)) * p.ldw;
-#pragma unroll
-    for (int i = 0; i < NT; ++i) {
-        xr[i] = p.xq + static_cast<size_t>(min(8 * i + g, p.n - 1)) * p.ldx;
-#pragma unroll
-        for (int j = 0; j < 2; ++j) sx[i][j] = p.xs + static_cast<size_t>(min(8 * i + 2 * t + j, p.n - 1)) * p.blocks;
+    for (int i = 0; i < 2; ++i) {
+        wr[i] = p.wq + static_cast<size_t>(min(row0 + g + 8 * i, p.m - 1)) * p.ldw;
+        sx[i] = p.xs + static_cast<size_t>(min(2 * t + i, p.n - 1)) * p.blocks;
     }
+    const uint8_t* xr = p.xq + static_cast<size_t>(min(g, p.n - 1)) * p.ldx;
     const float* sw = p.ws + static_cast<size_t>(row0 / kFp8Block) * p.blocks;
-    auto load = [&](StreamBlock<NT>& o, int kb) {
+    auto load = [&](StreamBlock& o, int kb) {
         if (kb >= p.blocks) return;
         const int c = kb * kFp8Block + 16 * t;
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
 #pragma unroll
             for (int i = 0; i < 2; ++i) o.a[i][h] = load_row16(wr[i], c + 64 * h, p.k);
-#pragma unroll
-            for (int i = 0; i < NT; ++i) o.b[i][h] = load_row16(xr[i], c + 64 * h, p.k);
+            o.b[h] = load_row16(xr, c + 64 * h, p.k);
         }
         const float w = sw[kb];
 #pragma unroll
-        for (int i = 0; i < NT; ++i)
-#pragma unroll
-            for (int j = 0; j < 2; ++j) o.s[i][j] = sx[i][j][kb] * w;
+        for (int j = 0; j < 2; ++j) o.s[j] = sx[j][kb] * w;
     };
-    float acc[NT][4];
+    float acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+    StreamBlock ring[kStreamDepth];
 #pragma unroll
-    for (int i = 0; i < NT; ++i)
+    for (int d = 0; d < kStreamDepth; ++d) load(ring[d], warp + d * warps);
+    for (int kb = warp; kb < p.blocks; kb += kStreamDepth * warps) {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) acc[i][j] = 0.0f;
-    StreamBlock<NT> ring[DEPTH];
-#pragma unroll
-    for (int d = 0; d < DEPTH; ++d) load(ring[d], warp + d * warps);
-    for (int kb = warp; kb < p.blocks; kb += DEPTH * warps) {
-#pragma unroll
-        for (int d = 0; d < DEPTH; ++d) {
+        for (int d = 0; d < kStreamDepth; ++d) {
             const int at = kb + d * warps;
             if (at < p.blocks) {
-                const StreamBlock<NT>& o = ring[d];
+                const StreamBlock& o = ring[d];
+                float c[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-                for (int i = 0; i < NT; ++i) {
-                    float c[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-                    for (int h = 0; h < 2; ++h) {
-                        mma_16x8x32(c, o.a[0][h].x, o.a[1][h].x, o.a[0][h].y, o.a[1][h].y, o.b[i][h].x, o.b[i][h].y);
-                        mma_16x8x32(c, o.a[0][h].z, o.a[1][h].z, o.a[0][h].w, o.a[1][h].w, o.b[i][h].z, o.b[i][h].w);
-                    }
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) acc[i][j] = fmaf(c[j], o.s[i][j & 1], acc[i][j]);
+                for (int h = 0; h < 2; ++h) {
+                    mma_16x8x32(c, o.a[0][h].x, o.a[1][h].x, o.a[0][h].y, o.a[1][h].y, o.b[h].x, o.b[h].y);
+                    mma_16x8x32(c, o.a[0][h].z, o.a[1][h].z, o.a[0][h].w, o.a[1][h].w, o.b[h].z, o.b[h].w);
                 }
-                load(ring[d], at + DEPTH * warps);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) acc[j] = fmaf(c[j], o.s[j & 1], acc[j]);
+                load(ring[d], at + kStreamDepth * warps);
             }
         }
     }
 #pragma unroll
-    for (int i = 0; i < NT; ++i)
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-            part[(warp * 16 + g + (j >> 1) * 8) * kPitch + 8 * i + 2 * t + (j & 1)] = acc[i][j];
+    for (int j = 0; j < 4; ++j) part[(warp * 16 + g + (j >> 1) * 8) * kPitch + 2 * t + (j & 1)] = acc[j];
     __syncthreads();
     const int step = p.mode == kGemvSwiGLU ? 2 : 1, outs = 16 / step, wide = p.m / step;
     T* y = static_cast<T*>(p.y);
@@ -674,45 +938,61 @@ __global__ void __launch_bounds__(512) linear_fp8_stream_kernel(const StreamPara
     }
 }
 
-template <int NT, int DEPTH, typename T>
-cudaError_t launch_stream_tiles(const StreamParams& p, int warps, cudaStream_t s) {
-    count_launch();
-    linear_fp8_stream_kernel<NT, DEPTH, T>
-        <<<(p.m - 1) / 16 + 1, 32 * warps, static_cast<size_t>(warps) * 16 * (NT * 8 + 1) * 4, s>>>(p);
-    return cudaGetLastError();
-}
-
 template <typename T>
 cudaError_t launch_stream(const StreamParams& p, int num_sms, cudaStream_t s) {
     // enough warps to cover a memory round trip with the CTAs an SM holds; more where the rows are few
     int warps = 4;
-    while (warps < 16 && 2 * warps <= p.blocks && static_cast<long long>(p.m / 16) * warps < 16ll * num_sms) warps *= 2;
-    if (p.n <= 8) return launch_stream_tiles<1, 4, T>(p, warps, s);
-    if (p.n <= 16) return launch_stream_tiles<2, 3, T>(p, warps, s);
-    return launch_stream_tiles<4, 2, T>(p, warps, s);
+    while (warps < kStreamWarps && 2 * warps <= p.blocks && static_cast<long long>(p.m / 16) * warps < 16ll * num_sms)
+        warps *= 2;
+    count_launch();
+    linear_fp8_stream_kernel<T><<<(p.m - 1) / 16 + 1, 32 * warps, 0, s>>>(p);
+    return cudaGetLastError();
 }
 
-constexpr int kStreamTokens = 32;  // most tokens of the streaming kernel
+constexpr int kFewTokens = 64;  // most tokens of the kernel with features on the lanes
 
 int cdiv(long long a, long long b) { return static_cast<int>((a + b - 1) / b); }
 
-}  // namespace
+template <int N, typename T>
+cudaError_t launch_few_tokens(LinearParams& p, const uint8_t* xq, size_t ldx, const uint8_t* wq, size_t ldw, int k,
+                              int num_sms, cudaStream_t s) {
+    using F = Few<N>;
+    p.tiles_n = 1;
+    p.tiles_m = cdiv(p.m, 128);
+    p.x_rows = N;
+    p.stage_bytes = F::kStage;
+    p.stages = std::min(kMaxStages, (kSmemLimit - 1024 - kBarBytes - F::kScaleBytes) / F::kStage);
+    p.split = 1;
+    while (p.split < kMaxSplit && static_cast<long long>(p.tiles_m) * p.split * 2 <= num_sms && p.split * 2 <= p.blocks)
+        p.split *= 2;
+    // A CTA of a split tile has few K-blocks and takes no more stages than those: several share an SM, so that the
+    // clusters run at once (36 clusters of 4 with an SM a CTA did not: 8.2 us where one wave takes half of that).
+    if (p.split > 1)
+        p.stages = std::min(p.stages, std::max(cdiv(p.blocks, p.split), cdiv(static_cast<long long>(p.n) * 512, F::kStage)));
+    CUtensorMap mx, mw;
+    cudaError_t e = make_byte_map(&mx, xq, p.n, k, ldx, N);
+    if (e == cudaSuccess) e = make_byte_map(&mw, wq, p.m, k, ldw, 128);
+    if (e != cudaSuccess) return e;
+    static std::atomic<unsigned long long> allowed{0};
+    const int grid = p.split > 1 ? p.tiles_m * p.split : std::min(p.tiles_m, num_sms);
+    return launch_linear(linear_fp8_few_kernel<N, T>, allowed, mx, mw, p, grid, F::kThreads, p.split,
+                         p.stages * F::kStage + F::kScaleBytes + kBarBytes + 1024, s);
+}
 
-cudaError_t launch_linear_fp8(int mode, int dtype, const uint8_t* xq, size_t ldx, const float* xs, const uint8_t* wq,
-                              size_t ldw, const float* ws, const float* bias, void* y, int n, int m, int k, int num_sms,
-                              cudaStream_t s) {
-    if (n <= kStreamTokens) {
-        const StreamParams p{xq, wq, ldx, ldw, xs, ws, bias, y, mode, n, m, k, cdiv(k, kFp8Block)};
-        switch (dtype) {
-            case kF32: return launch_stream<float>(p, num_sms, s);
-            case kBF16: return launch_stream<__nv_bfloat16>(p, num_sms, s);
-            case kF16: return launch_stream<__half>(p, num_sms, s);
-            default: return cudaErrorInvalidValue;
-        }
+template <typename T>
+cudaError_t launch_tokens(LinearParams& p, const uint8_t* xq, size_t ldx, const uint8_t* wq, size_t ldw, int k, int num_sms,
+                          cudaStream_t s) {
+    const int n = p.n, m = p.m;
+    // One memory round trip through registers, or TMA, tcgen05 and (split) a cluster's exchange: 8 tokens take 4.2 us
+    // against 5.7 for 4608 x 1536 weights (7.1 MB), 7.0 against 5.6 for 8192 x 1536 (12.6 MB); 16 tokens would take
+    // 6.3 against 5.9 and 11.0 against 5.9.
+    if (n <= kStreamTokens && static_cast<long long>(m) * k <= kStreamBytes) {
+        const StreamParams sp{xq, wq, ldx, ldw, p.xs, p.ws, p.bias, p.y, p.mode, n, m, k, p.blocks};
+        return launch_stream<T>(sp, num_sms, s);
     }
-    LinearParams p{};
-    p.xs = xs, p.ws = ws, p.bias = bias, p.y = y;
-    p.mode = mode, p.n = n, p.m = m, p.blocks = cdiv(k, kFp8Block);
+    if (n <= 16) return launch_few_tokens<16, T>(p, xq, ldx, wq, ldw, k, num_sms, s);
+    if (n <= 32) return launch_few_tokens<32, T>(p, xq, ldx, wq, ldw, k, num_sms, s);
+    if (n <= kFewTokens) return launch_few_tokens<64, T>(p, xq, ldx, wq, ldw, k, num_sms, s);
     // Rounds of K-blocks either tiling takes: a K-block costs about the same
     // time in both (operands from L2), a pair's covers four times the outputs.
     const long long t1 = static_cast<long long>(cdiv(n, 128)) * cdiv(m, 128);
@@ -737,14 +1017,21 @@ cudaError_t launch_linear_fp8(int mode, int dtype, const uint8_t* xq, size_t ldx
     const long long tiles = static_cast<long long>(p.tiles_n) * p.tiles_m;
     const int grid = pair ? 2 * static_cast<int>(std::min<long long>(tiles, num_sms / 2))
                           : p.split * static_cast<int>(p.split > 1 ? tiles : std::min<long long>(tiles, num_sms));
-    auto go = [&](auto t) {
-        using T = decltype(t);
-        return pair ? launch_tiled<2, T>(mx, mw, p, grid, s) : launch_tiled<1, T>(mx, mw, p, grid, s);
-    };
+    return pair ? launch_tiled<2, T>(mx, mw, p, grid, s) : launch_tiled<1, T>(mx, mw, p, grid, s);
+}
+
+}  // namespace
+
+cudaError_t launch_linear_fp8(int mode, int dtype, const uint8_t* xq, size_t ldx, const float* xs, const uint8_t* wq,
+                              size_t ldw, const float* ws, const float* bias, void* y, int n, int m, int k, int num_sms,
+                              cudaStream_t s) {
+    LinearParams p{};
+    p.xs = xs, p.ws = ws, p.bias = bias, p.y = y;
+    p.mode = mode, p.n = n, p.m = m, p.blocks = cdiv(k, kFp8Block);
     switch (dtype) {
-        case kF32: return go(float{});
-        case kBF16: return go(__nv_bfloat16{});
-        case kF16: return go(__half{});
+        case kF32: return launch_tokens<float>(p, xq, ldx, wq, ldw, k, num_sms, s);
+        case kBF16: return launch_tokens<__nv_bfloat16>(p, xq, ldx, wq, ldw, k, num_sms, s);
+        case kF16: return launch_tokens<__half>(p, xq, ldx, wq, ldw, k, num_sms, s);
         default: return cudaErrorInvalidValue;
     }
 }
