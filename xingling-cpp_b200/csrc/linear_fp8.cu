@@ -3,26 +3,21 @@
 //   Y[i][j] = sum_b sx[i][b] sw[j / 128][b] sum_{c in block b} xq[i][c] wq[j][c] + bias[j]
 //
 // A K-block is one scale block: 128 columns = 128 bytes, the SWIZZLE_128B span.
-// Tokens are the MMA's M (TMEM lanes), features its N (TMEM columns): a thread
-// of the epilogue then holds one token, for which sx sw is one number for all
-// features of a 128-block, so scaling a K-block's sum into the fp32 result is
-// one multiply-add per value with no loads.  The tensor core sums within a
-// block (products of e4m3 values are exact in fp32), registers across blocks.
+// The tensor core sums within a block (products of e4m3 values are exact in
+// fp32), registers across blocks, each block's sum scaled in with one
+// multiply-add.  One warp issues TMA loads into a ring of stages, one the MMAs
+// of a K-block into the next of several TMEM accumulators, the others drain
+// them; the accumulators decouple the two.
 //
-// One warp issues TMA loads into a ring of stages, one thread the MMAs of a
-// K-block into the next of several TMEM accumulators, 4 or 8 warps drain
-// them; the accumulators decouple the two, so the tensor core only waits for
-// operands.
-//
-// Two tilings:
-//   * 128 tokens x 128 features on one SM; fewer tiles than SMs split K over
-//     the CTAs of a cluster, whose partial tiles meet in distributed shared
-//     memory, each CTA finishing a share of the columns (a fixed order of
-//     sums, no workspace).  Few tokens load few rows: the rest of the A tile
-//     is whatever the stage holds, and only its own (unread) lanes see it.
-//   * 256 x 256 on two SMs (cta_group::2), each with half of either operand:
-//     64 bytes a clock from L2 per SM where a 128 x 256 tile on one SM needs
-//     96, twice the reuse of the 128 x 128 tile.
+// Three kernels:
+//   * large products: 256 tokens x 256 features on two SMs (cta_group::2),
+//     each with half of either operand, which asks 64 bytes a clock of L2 per
+//     SM where 128 x 256 on one SM asks 96.  Tokens are the MMA's M (TMEM
+//     lanes): a thread holds one token, for which sx sw is one number for all
+//     features of a 128-block;
+//   * few tokens or few tiles: 128 features (lanes) x 16 to 128 tokens
+//     (columns) on one SM, K split over a cluster where tiles are few;
+//   * 8 tokens and few weights: registers and mma.sync, one memory round trip.
 #include <cuda.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -39,24 +34,22 @@ namespace xl {
 
 namespace {
 
-constexpr int kRows = 128;                   // token rows of a CTA's A tile
-constexpr int kOpBytes = 128 * kFp8Block;    // 16 KB: 128 rows of a K-block
+constexpr int kOpBytes = 128 * kFp8Block;    // 16 KB: 128 rows of an operand's K-block
 constexpr int kMaxStages = 12;
 constexpr int kMaxSplit = 8;                 // portable cluster size
 constexpr int kStagePitch = 20;              // floats a row of the store staging: 16 and padding, conflict-free in float4
 constexpr int kSmemLimit = 232448;           // 227 KB
 constexpr int kBarBytes = 512;
-constexpr int kPartPitch = kRows + 1;        // split: partial tile [128 features][129]
 
-template <int CG>
-struct Tile {
-    static constexpr int kTokens = CG * kRows;          // of the tile, all CTAs
-    static constexpr int kFeatures = CG * 128;          // each CTA loads 128 of them
-    static constexpr int kEpiWarps = 4 * CG;            // each drains 32 lanes x 128 columns
-    // two issuing warps (the pair's tiling: a warpgroup, so that registers can be moved to the epilogue's)
-    static constexpr int kEpiFirst = CG == 1 ? 2 : 4;
+// 256 tokens x 256 features on a pair of SMs.
+struct Pair {
+    static constexpr int kTokens = 256, kFeatures = 256;  // of the tile; each CTA loads 128 of either
+    static constexpr int kStage = 2 * kOpBytes;
+    static constexpr int kEpiWarps = 8;                   // each drains 32 lanes x 128 columns
+    // the issuing warps are a warpgroup, so that registers can be moved to the epilogue's two
+    static constexpr int kEpiFirst = 4;
     static constexpr int kThreads = 32 * (kEpiFirst + kEpiWarps);
-    static constexpr int kAccs = 512 / kFeatures;       // TMEM accumulators
+    static constexpr int kAccs = 512 / kFeatures;         // TMEM accumulators
     static constexpr int kWarpStore = 32 * kStagePitch + 128;  // floats: a warp's staging rows and its bias
     static constexpr int kStoreBytes = kEpiWarps * kWarpStore * 4;
     // kind::f8f6f4, e4m3 x e4m3, fp32 sums, K-major operands
@@ -68,9 +61,8 @@ struct LinearParams {
     const float *xs, *ws, *bias;
     void* y;
     int mode, n, m, blocks;     // blocks: K-blocks
-    int x_rows;                 // token rows a CTA loads (a multiple of 8, at most 128)
-    int stages, stage_bytes;
-    int split;                  // CTAs of a cluster that share a tile's K-blocks (one-SM tiling)
+    int stages;
+    int split;                  // CTAs of a cluster that share a tile's K-blocks (features on lanes)
     int tiles_n, tiles_m;
 };
 
@@ -264,92 +256,77 @@ __device__ __forceinline__ void store_rows(const unsigned long long (&acc)[64], 
     }
 }
 
-template <int CG, typename T>
-__global__ void __launch_bounds__(Tile<CG>::kThreads, 1)
-    linear_fp8_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_w,
-                      const LinearParams p) {
-    using TL = Tile<CG>;
+template <typename T>
+__global__ void __launch_bounds__(Pair::kThreads, 1)
+    linear_fp8_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_w,
+                           const LinearParams p) {
     extern __shared__ __align__(1024) char smem_raw[];
     char* ring = reinterpret_cast<char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
-    float* store = reinterpret_cast<float*>(ring + p.stages * p.stage_bytes);
-    uint64_t* full = reinterpret_cast<uint64_t*>(reinterpret_cast<char*>(store) + TL::kStoreBytes);
+    float* store = reinterpret_cast<float*>(ring + p.stages * Pair::kStage);
+    uint64_t* full = reinterpret_cast<uint64_t*>(reinterpret_cast<char*>(store) + Pair::kStoreBytes);
     uint64_t* empty = full + kMaxStages;
-    uint64_t* done = empty + kMaxStages;  // an accumulator holds a K-block's sums
-    uint64_t* freed = done + TL::kAccs;   // its columns have been read
-    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(freed + TL::kAccs);
+    uint64_t* done = empty + kMaxStages;   // an accumulator holds a K-block's sums
+    uint64_t* freed = done + Pair::kAccs;  // its columns have been read, in both CTAs
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(freed + Pair::kAccs);
 
     const int warp = __shfl_sync(0xffffffffu, static_cast<int>(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
-    const uint32_t rank = CG == 2 || p.split > 1 ? cluster_rank() : 0u;
-    const int group = CG == 2 ? 2 : p.split;  // CTAs that share a tile
-    const int unit = static_cast<int>(blockIdx.x) / group, units = static_cast<int>(gridDim.x) / group;
+    const int rank = static_cast<int>(cluster_rank());
+    const int unit = static_cast<int>(blockIdx.x) / 2, units = static_cast<int>(gridDim.x) / 2;
     const int tiles = p.tiles_n * p.tiles_m;
-    const int kb0 = CG == 2 ? 0 : static_cast<int>(static_cast<long long>(rank) * p.blocks / p.split);
-    const int kb1 = CG == 2 ? p.blocks : static_cast<int>(static_cast<long long>(rank + 1) * p.blocks / p.split);
 
-    if (threadIdx.x == 0) {
-        for (int s = 0; s < p.stages; ++s) {
-            mbar_init(&full[s], 1);
-            mbar_init(&empty[s], 1);
+    if (warp == 0) {
+        if (elect_one()) asm volatile("prefetch.tensormap [%0];\n\tprefetch.tensormap [%1];" ::"l"(&map_x), "l"(&map_w) : "memory");
+        if (lane < p.stages) {
+            mbar_init(&full[lane], 1);
+            mbar_init(&empty[lane], 1);
         }
-        for (int a = 0; a < TL::kAccs; ++a) {
-            mbar_init(&done[a], 1);
-            mbar_init(&freed[a], CG * TL::kEpiWarps);
+        if (lane < Pair::kAccs) {
+            mbar_init(&done[lane], 1);
+            mbar_init(&freed[lane], 2 * Pair::kEpiWarps);
         }
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-        asm volatile("prefetch.tensormap [%0];\n\tprefetch.tensormap [%1];" ::"l"(&map_x), "l"(&map_w) : "memory");
     }
     if (warp == 1) {
-        if (CG == 1) {
-            asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(tmem_slot))
-                         : "memory");
-            asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
-        } else {
-            asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(tmem_slot))
-                         : "memory");
-            asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
-        }
+        asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(tmem_slot))
+                     : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
     }
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
     __syncthreads();
-    if (CG == 2) cluster_sync();  // the peer's barriers are set up before anything arrives on them
+    cluster_sync();  // the peer's barriers are set up before anything arrives on them
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
     const uint32_t tmem = *tmem_slot;
 
-    // Token tiles advance fastest: the CTAs that run together share W tiles
-    // and, over the whole product, either operand stays in L2.
-    const uint32_t a_bytes = static_cast<uint32_t>(p.x_rows) * kFp8Block;
-    // The pair's epilogue needs 128 sums and 64 columns in flight a thread: 384 threads launch with 168
-    // registers, the issuing warpgroup keeps 40, the others take 232 (128 x 40 + 256 x 232 = 384 x 168).
-    if (CG == 2 && warp < TL::kEpiFirst) asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
-    // Both issuing warps run their loops converged and elect one lane to issue.
+    // The epilogue needs 128 sums and 64 columns in flight a thread: 384 threads launch with 168 registers, the
+    // issuing warpgroup keeps 40, the others take 232 (128 x 40 + 256 x 232 = 384 x 168).
+    if (warp < Pair::kEpiFirst) asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
+    // Token tiles advance fastest: the CTAs that run together share W tiles and, over the whole product, either
+    // operand stays in L2.  Both issuing warps run their loops converged and elect one lane to issue.
     if (warp == 0) {
         int s = 0;
         uint32_t ph = 0, issued = 0;
         bool ok = true;
+        const uint32_t bar0 = cluster_addr(smem_u32(full), 0);  // both CTAs' copies are counted in the first one
         for (int t = unit; t < tiles && ok; t += units) {
-            const int tn = t % p.tiles_n, tm = t / p.tiles_n;
-            const int y_x = tn * TL::kTokens + (CG == 2 ? static_cast<int>(rank) * kRows : 0);
-            const int y_w = tm * TL::kFeatures + (CG == 2 ? static_cast<int>(rank) * 128 : 0);
-            for (int kb = kb0; kb < kb1; ++kb) {
+            const int y_x = t % p.tiles_n * Pair::kTokens + rank * 128, y_w = t / p.tiles_n * Pair::kFeatures + rank * 128;
+            for (int kb = 0; kb < p.blocks; ++kb) {
                 if (!wait_warp(&empty[s], ph ^ 1u)) {
                     ok = false;
                     break;
                 }
-                const uint32_t st = smem_u32(ring + s * p.stage_bytes);
-                uint32_t bar = smem_u32(&full[s]);
-                if (CG == 2) bar = cluster_addr(bar, 0);
+                const uint32_t st = smem_u32(ring + s * Pair::kStage);
                 if (elect_one()) {
-                    if (CG == 1 || rank == 0) mbar_expect_tx(&full[s], CG * (a_bytes + kOpBytes));
-                    load_tile<CG>(st + a_bytes, &map_w, kb * kFp8Block, y_w, bar);
-                    load_tile<CG>(st, &map_x, kb * kFp8Block, y_x, bar);
+                    if (rank == 0) mbar_expect_tx(&full[s], 2 * Pair::kStage);
+                    load_tile<2>(st, &map_x, kb * kFp8Block, y_x, bar0 + 8 * s);
+                    load_tile<2>(st + kOpBytes, &map_w, kb * kFp8Block, y_w, bar0 + 8 * s);
                 }
                 __syncwarp();
                 ++issued;
                 if (++s == p.stages) s = 0, ph ^= 1u;
             }
         }
-        if (!ok && (CG == 1 || rank == 0)) {
-            // the copies in flight land before the CTA leaves
+        if (!ok && rank == 0) {
+            // the copies in flight land before the CTAs leave
             for (uint32_t i = 0; i < min(issued, static_cast<uint32_t>(p.stages)); ++i) {
                 if (s == 0) s = p.stages, ph ^= 1u;
                 --s;
@@ -357,47 +334,46 @@ __global__ void __launch_bounds__(Tile<CG>::kThreads, 1)
             }
         }
     } else if (warp == 1) {
-        if (CG == 1 || rank == 0) {
+        if (rank == 0) {
             int s = 0, a = 0;
             uint32_t ph = 0, pa = 0;
             bool ok = true;
             for (int t = unit; t < tiles && ok; t += units) {
-                for (int kb = kb0; kb < kb1; ++kb) {
-                    if (!wait_warp(&freed[a], pa ^ 1u) || !wait_warp(&full[s], ph)) {
+                for (int kb = 0; kb < p.blocks; ++kb) {
+                    if (!wait_warp(&full[s], ph) || !wait_warp(&freed[a], pa ^ 1u)) {
                         ok = false;
                         break;
                     }
                     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                    const uint32_t st = smem_u32(ring + s * p.stage_bytes);
-                    const uint64_t da = umma_desc(st), db = umma_desc(st + a_bytes);
-                    const uint32_t acc = tmem + static_cast<uint32_t>(a * TL::kFeatures);
+                    const uint32_t st = smem_u32(ring + s * Pair::kStage);
+                    const uint64_t dx = umma_desc(st), dw = umma_desc(st + kOpBytes);
+                    const uint32_t acc = tmem + static_cast<uint32_t>(a * Pair::kFeatures);
                     if (elect_one()) {
 #pragma unroll
                         for (int ks = 0; ks < 4; ++ks)  // 32 columns = 32 bytes each
-                            mma_e4m3<CG>(acc, da + 2 * ks, db + 2 * ks, TL::kIdesc, ks != 0);
-                        commit<CG>(&empty[s]);
-                        commit<CG>(&done[a]);
+                            mma_e4m3<2>(acc, dx + 2 * ks, dw + 2 * ks, Pair::kIdesc, ks != 0);
+                        commit<2>(&done[a]);
+                        commit<2>(&empty[s]);
                     }
                     __syncwarp();
                     if (++s == p.stages) s = 0, ph ^= 1u;
-                    if (++a == TL::kAccs) a = 0, pa ^= 1u;
+                    if (++a == Pair::kAccs) a = 0, pa ^= 1u;
                 }
             }
         }
-    } else if (warp >= TL::kEpiFirst) {
-        if (CG == 2) asm volatile("setmaxnreg.inc.sync.aligned.u32 232;");
+    } else if (warp >= Pair::kEpiFirst) {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 232;");
         // TMEM lanes are a warp's by its number modulo 4
-        const int q = warp & 3, half = (warp - TL::kEpiFirst) >> 2;
-        float* st = store + (warp - TL::kEpiFirst) * TL::kWarpStore;
+        const int q = warp & 3, half = (warp - Pair::kEpiFirst) >> 2;
+        float* st = store + (warp - Pair::kEpiFirst) * Pair::kWarpStore;
         float* sb = st + 32 * kStagePitch;
         int a = 0;
         uint32_t pa = 0;
         bool ok = true;
-        const uint32_t freed0 = CG == 2 ? cluster_addr(smem_u32(freed), 0) : smem_u32(freed);
+        const uint32_t freed0 = cluster_addr(smem_u32(freed), 0);
         for (int t = unit; t < tiles; t += units) {
-            const int tn = t % p.tiles_n, tm = t / p.tiles_n;
-            const int tok0 = tn * TL::kTokens + (CG == 2 ? static_cast<int>(rank) * kRows : 0) + 32 * q;
-            const int j0 = tm * TL::kFeatures + 128 * half;
+            const int tok0 = t % p.tiles_n * Pair::kTokens + rank * 128 + 32 * q;
+            const int j0 = t / p.tiles_n * Pair::kFeatures + 128 * half;
             const bool work = tok0 < p.n && j0 < p.m;  // else the warp only keeps the accumulators moving
             const float* xs = p.xs + static_cast<size_t>(min(tok0 + lane, p.n - 1)) * p.blocks;
             const float* ws = p.ws + static_cast<size_t>(min(j0, p.m - 1) / kFp8Block) * p.blocks;
@@ -410,12 +386,12 @@ __global__ void __launch_bounds__(Tile<CG>::kThreads, 1)
             unsigned long long acc[64];
 #pragma unroll
             for (int i = 0; i < 64; ++i) acc[i] = 0;
-            float sx = xs[kb0], sw = ws[kb0];
-            bool ready = mbar_try_wait(&done[a], pa);
+            float sx = xs[0], sw = ws[0];
+            bool ready = mbar_test_wait(&done[a], pa);
 #pragma unroll 1
-            for (int kb = kb0; kb < kb1; ++kb) {
+            for (int kb = 0; kb < p.blocks; ++kb) {
                 const float s = sx * sw;
-                const int next = min(kb + 1, kb1 - 1);
+                const int next = min(kb + 1, p.blocks - 1);
                 sx = xs[next], sw = ws[next];
                 if (ok && !__all_sync(0xffffffffu, ready)) ok = wait_warp(&done[a], pa);
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
@@ -424,7 +400,7 @@ __global__ void __launch_bounds__(Tile<CG>::kThreads, 1)
                 uint32_t r0[32], r1[32];
                 if (drain) {
                     const uint32_t ta = tmem + (static_cast<uint32_t>(32 * q) << 16) +
-                                        static_cast<uint32_t>(a * TL::kFeatures + 128 * half);
+                                        static_cast<uint32_t>(a * Pair::kFeatures + 128 * half);
                     // two rounds of 64 columns in flight; the accumulator is handed back before the last sums
                     tmem_load32(ta, r0);
                     tmem_load32(ta + 32, r1);
@@ -441,8 +417,8 @@ __global__ void __launch_bounds__(Tile<CG>::kThreads, 1)
                     // only TMEM reads are ordered by this arrival (the fence above); a cluster-wide release of
                     // memory would cost over 1000 clocks a K-block
                     asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(freed0 + 8 * a) : "memory");
-                if (++a == TL::kAccs) a = 0, pa ^= 1u;
-                if (kb + 1 < kb1) ready = mbar_try_wait(&done[a], pa);  // asked early: the answer comes behind the sums
+                if (++a == Pair::kAccs) a = 0, pa ^= 1u;
+                if (kb + 1 < p.blocks) ready = mbar_test_wait(&done[a], pa);  // asked early: the answer comes behind the sums
                 if (drain) {
                     scale_in(acc, 32, r0, s2);
                     scale_in(acc, 48, r1, s2);
@@ -452,62 +428,21 @@ __global__ void __launch_bounds__(Tile<CG>::kThreads, 1)
 #pragma unroll
                 for (int i = 0; i < 64; ++i) acc[i] = 0x7fffffff7fffffffull;
             }
-            if (CG == 2 || p.split == 1) {
-                if (work) {
+            if (work) {
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) sb[32 * i + lane] = bias[i];
-                    __syncwarp();
-                    store_rows<T>(acc, p, tok0, j0, st, reinterpret_cast<const float4*>(sb), lane);
-                }
-            } else {
-                // every K-block of this CTA has been multiplied: the ring is free for the partial tile
-                float* part = reinterpret_cast<float*>(ring);
-                if (work && tok0 + lane < p.n) {
-#pragma unroll
-                    for (int i = 0; i < 64; ++i) {
-                        const float2 v = unpack2(acc[i]);
-                        part[(2 * i) * kPartPitch + 32 * q + lane] = v.x;
-                        part[(2 * i + 1) * kPartPitch + 32 * q + lane] = v.y;
-                    }
-                }
+                for (int i = 0; i < 4; ++i) sb[32 * i + lane] = bias[i];
+                __syncwarp();
+                store_rows<T>(acc, p, tok0, j0, st, reinterpret_cast<const float4*>(sb), lane);
             }
         }
         asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
     }
-    if (CG == 1 && p.split > 1) {
-        __syncwarp();
-        cluster_sync();
-        // A cluster has one tile; this CTA finishes 128 / split of its columns.
-        const int tn = unit % p.tiles_n, tm = unit / p.tiles_n;
-        const int rows = min(kRows, p.n - tn * kRows), step = p.mode == kGemvSwiGLU ? 2 : 1;
-        const int cols = 128 / p.split, outs = cols / step, wide = p.m / step;
-        const uint32_t part = smem_u32(ring);
-        T* y = static_cast<T*>(p.y);
-        for (int e = threadIdx.x; e < rows * outs; e += TL::kThreads) {
-            const int r = e / outs, c = static_cast<int>(rank) * cols + (e - r * outs) * step, j = tm * 128 + c;
-            if (j >= p.m) continue;
-            float v[2] = {0.0f, 0.0f};
-            for (int i = 0; i < step; ++i) {
-                const uint32_t at = part + static_cast<uint32_t>((c + i) * kPartPitch + r) * 4;
-                for (int k = 0; k < p.split; ++k) {
-                    float x;
-                    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(x) : "r"(cluster_addr(at, k)) : "memory");
-                    v[i] += x;
-                }
-                if (p.bias) v[i] += p.bias[j + i];
-            }
-            put(y + static_cast<size_t>(tn * kRows + r) * wide + j / step, step == 2 ? silu_fast(v[0]) * v[1] : v[0], p.mode);
-        }
-    }
     __syncwarp();
     __syncthreads();
-    if (CG == 2 || p.split > 1) cluster_sync();  // no CTA leaves while another may reach its shared memory
+    cluster_sync();  // no CTA leaves while the other may reach its shared memory
     if (warp == 1) {
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-        if (CG == 1)
-            asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
-        else
-            asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
+        asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
     }
 }
 
@@ -541,27 +476,24 @@ cudaError_t launch_linear(LinearKernel kernel, std::atomic<unsigned long long>& 
     return cudaLaunchKernelEx(&cfg, kernel, mx, mw, p);
 }
 
-template <int CG, typename T>
-cudaError_t launch_tiled(const CUtensorMap& mx, const CUtensorMap& mw, const LinearParams& p, int grid, cudaStream_t s) {
-    using TL = Tile<CG>;
-    if (CG == 2) {
-        // the warpgroups' register shares have to fit what the CTA launches with, or the larger one never comes
-        static const bool fits = [] {
-            cudaFuncAttributes a{};
-            return cudaFuncGetAttributes(&a, linear_fp8_kernel<CG, T>) == cudaSuccess &&
-                   a.numRegs * TL::kThreads >= 128 * 40 + 256 * 232;
-        }();
-        if (!fits) return cudaErrorInvalidConfiguration;
-    }
+template <typename T>
+cudaError_t launch_pairs(const CUtensorMap& mx, const CUtensorMap& mw, const LinearParams& p, int grid, cudaStream_t s) {
+    // the warpgroups' register shares have to fit what the CTA launches with, or the larger one never comes
+    static const bool fits = [] {
+        cudaFuncAttributes a{};
+        return cudaFuncGetAttributes(&a, linear_fp8_pair_kernel<T>) == cudaSuccess &&
+               a.numRegs * Pair::kThreads >= 128 * 40 + 256 * 232;
+    }();
+    if (!fits) return cudaErrorInvalidConfiguration;
     static std::atomic<unsigned long long> allowed{0};
-    return launch_linear(linear_fp8_kernel<CG, T>, allowed, mx, mw, p, grid, TL::kThreads, CG == 2 ? 2 : p.split,
-                         p.stages * p.stage_bytes + TL::kStoreBytes + kBarBytes + 1024, s);
+    return launch_linear(linear_fp8_pair_kernel<T>, allowed, mx, mw, p, grid, Pair::kThreads, 2,
+                         p.stages * Pair::kStage + Pair::kStoreBytes + kBarBytes + 1024, s);
 }
 
-// ---- up to 64 tokens: features on the TMEM lanes ----
+// ---- few tokens or tiles: features on the TMEM lanes ----
 //
 // The operands change places: 128 features are the MMA's M, the tokens its N
-// (16, 32 or 64).  A K-block then leaves few columns to drain, a lane's
+// (16 to 128).  A K-block then leaves few columns to drain, a lane's
 // results of one token lie next to its neighbours' in y, and the tensor core
 // takes a K-block in the time its weights take to arrive.  Fewer tiles than
 // SMs split K over the CTAs of a cluster, whose partial tiles meet in
@@ -569,8 +501,10 @@ cudaError_t launch_tiled(const CUtensorMap& mx, const CUtensorMap& mw, const Lin
 
 template <int N>
 struct Few {
-    static constexpr int kAccs = N == 64 ? 4 : 8;
+    static constexpr int kAccs = N >= 64 ? 4 : 8;
     static constexpr int kColumns = kAccs * N;
+    static constexpr int kRound = N < 64 ? N : 64;     // columns drained at a time
+    static constexpr int kCtas = N == 128 ? 1 : 2;     // an SM holds at least, by registers
     static constexpr int kThreads = 192;
     static constexpr int kStage = kOpBytes + N * kFp8Block;
     static constexpr int kScaleBytes = 4 * N * 4;  // a warp's N scales
@@ -595,7 +529,7 @@ __device__ __forceinline__ void tmem_wait16(uint32_t* r) {
 }
 
 template <int N, typename T>
-__global__ void __launch_bounds__(Few<N>::kThreads, 2)
+__global__ void __launch_bounds__(Few<N>::kThreads, Few<N>::kCtas)
     linear_fp8_few_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_w,
                           const LinearParams p) {
     using F = Few<N>;
@@ -611,6 +545,7 @@ __global__ void __launch_bounds__(Few<N>::kThreads, 2)
     const int warp = __shfl_sync(0xffffffffu, static_cast<int>(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
     const uint32_t rank = p.split > 1 ? cluster_rank() : 0u;
     const int unit = static_cast<int>(blockIdx.x) / p.split, units = static_cast<int>(gridDim.x) / p.split;
+    const int tiles = p.tiles_n * p.tiles_m;
     const int kb0 = static_cast<int>(static_cast<long long>(rank) * p.blocks / p.split);
     const int kb1 = static_cast<int>(static_cast<long long>(rank + 1) * p.blocks / p.split);
 
@@ -641,7 +576,8 @@ __global__ void __launch_bounds__(Few<N>::kThreads, 2)
         int s = 0;
         uint32_t ph = 0, issued = 0;
         bool ok = true;
-        for (int t = unit; t < p.tiles_m && ok; t += units) {
+        for (int t = unit; t < tiles && ok; t += units) {
+            const int tn = t % p.tiles_n, tm = t / p.tiles_n;
             for (int kb = kb0; kb < kb1; ++kb) {
                 if (!wait_warp(&empty[s], ph ^ 1u)) {
                     ok = false;
@@ -650,8 +586,8 @@ __global__ void __launch_bounds__(Few<N>::kThreads, 2)
                 const uint32_t st = smem_u32(ring + s * F::kStage);
                 if (elect_one()) {
                     mbar_expect_tx(&full[s], F::kStage);
-                    load_tile<1>(st, &map_w, kb * kFp8Block, t * 128, smem_u32(&full[s]));
-                    load_tile<1>(st + kOpBytes, &map_x, kb * kFp8Block, 0, smem_u32(&full[s]));
+                    load_tile<1>(st, &map_w, kb * kFp8Block, tm * 128, smem_u32(&full[s]));
+                    load_tile<1>(st + kOpBytes, &map_x, kb * kFp8Block, tn * N, smem_u32(&full[s]));
                 }
                 __syncwarp();
                 ++issued;
@@ -670,7 +606,7 @@ __global__ void __launch_bounds__(Few<N>::kThreads, 2)
         int s = 0, a = 0;
         uint32_t ph = 0, pa = 0;
         bool ok = true;
-        for (int t = unit; t < p.tiles_m && ok; t += units) {
+        for (int t = unit; t < tiles && ok; t += units) {
             for (int kb = kb0; kb < kb1; ++kb) {
                 if (!wait_warp(&freed[a], pa ^ 1u) || !wait_warp(&full[s], ph)) {
                     ok = false;
@@ -697,52 +633,59 @@ __global__ void __launch_bounds__(Few<N>::kThreads, 2)
         int a = 0;
         uint32_t pa = 0;
         bool ok = true;
-        const float* xs[N / 32 + 1];
+        constexpr int kLots = (N + 31) / 32;
+        for (int t = unit; t < tiles; t += units) {
+            const int tok0 = t % p.tiles_n * N, tm = t / p.tiles_n, rows = min(N, p.n - tok0);
+            const float* xs[kLots];
 #pragma unroll
-        for (int i = 0; i < (N + 31) / 32; ++i) xs[i] = p.xs + static_cast<size_t>(min(32 * i + lane, p.n - 1)) * p.blocks;
-        for (int t = unit; t < p.tiles_m; t += units) {
-            const float* ws = p.ws + static_cast<size_t>(t) * p.blocks;
-            const int j = t * 128 + 32 * q + lane;
+            for (int i = 0; i < kLots; ++i) xs[i] = p.xs + static_cast<size_t>(min(tok0 + 32 * i + lane, p.n - 1)) * p.blocks;
+            const float* ws = p.ws + static_cast<size_t>(tm) * p.blocks;
+            const int j = tm * 128 + 32 * q + lane;
             const float bias = p.bias && j < p.m ? p.bias[j] : 0.0f;
             unsigned long long acc[N / 2];
 #pragma unroll
             for (int i = 0; i < N / 2; ++i) acc[i] = 0;
-            float sx[(N + 31) / 32], sw = ws[kb0];
+            float sx[kLots], sw = ws[kb0];
 #pragma unroll
-            for (int i = 0; i < (N + 31) / 32; ++i) sx[i] = xs[i][kb0];
-            bool ready = mbar_try_wait(&done[a], pa);
+            for (int i = 0; i < kLots; ++i) sx[i] = xs[i][kb0];
+            bool ready = mbar_test_wait(&done[a], pa);
 #pragma unroll 1
             for (int kb = kb0; kb < kb1; ++kb) {
 #pragma unroll
-                for (int i = 0; i < (N + 31) / 32; ++i)
+                for (int i = 0; i < kLots; ++i)
                     if (32 * i + lane < N) sc[32 * i + lane] = sx[i] * sw;
                 const int next = min(kb + 1, kb1 - 1);
                 sw = ws[next];
 #pragma unroll
-                for (int i = 0; i < (N + 31) / 32; ++i) sx[i] = xs[i][next];
+                for (int i = 0; i < kLots; ++i) sx[i] = xs[i][next];
                 __syncwarp();
                 if (ok && !__all_sync(0xffffffffu, ready)) ok = wait_warp(&done[a], pa);
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                uint32_t r[N];
+                uint32_t r[F::kRound];
                 const uint32_t ta = tmem + (static_cast<uint32_t>(32 * q) << 16) + static_cast<uint32_t>(a * N);
-                if (ok) {
 #pragma unroll
-                    for (int i = 0; i < N; i += 16) tmem_load16(ta + i, r + i);
+                for (int c = 0; c < N; c += F::kRound) {
+                    if (ok) {
 #pragma unroll
-                    for (int i = 0; i < N; i += 16) tmem_wait16(r + i);
-                }
-                asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-                __syncwarp();
-                if (elect_one())
-                    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(&freed[a])) : "memory");
-                if (++a == F::kAccs) a = 0, pa ^= 1u;
-                if (kb + 1 < kb1) ready = mbar_try_wait(&done[a], pa);
-                if (ok) {
+                        for (int i = 0; i < F::kRound; i += 16) tmem_load16(ta + c + i, r + i);
 #pragma unroll
-                    for (int i = 0; i < N / 4; ++i) {
-                        const ulonglong2 s4 = reinterpret_cast<const ulonglong2*>(sc)[i];
-                        fma2(acc[2 * i], pack2(r[4 * i], r[4 * i + 1]), s4.x);
-                        fma2(acc[2 * i + 1], pack2(r[4 * i + 2], r[4 * i + 3]), s4.y);
+                        for (int i = 0; i < F::kRound; i += 16) tmem_wait16(r + i);
+                    }
+                    if (c + F::kRound == N) {  // handed back before the last sums
+                        asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+                        __syncwarp();
+                        if (elect_one())
+                            asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(&freed[a])) : "memory");
+                        if (++a == F::kAccs) a = 0, pa ^= 1u;
+                        if (kb + 1 < kb1) ready = mbar_test_wait(&done[a], pa);
+                    }
+                    if (ok) {
+#pragma unroll
+                        for (int i = 0; i < F::kRound / 4; ++i) {
+                            const ulonglong2 s4 = reinterpret_cast<const ulonglong2*>(sc)[c / 4 + i];
+                            fma2(acc[c / 2 + 2 * i], pack2(r[4 * i], r[4 * i + 1]), s4.x);
+                            fma2(acc[c / 2 + 2 * i + 1], pack2(r[4 * i + 2], r[4 * i + 3]), s4.y);
+                        }
                     }
                 }
                 __syncwarp();
@@ -756,14 +699,15 @@ __global__ void __launch_bounds__(Few<N>::kThreads, 2)
                 const bool swiglu = p.mode == kGemvSwiGLU;
 #pragma unroll
                 for (int i = 0; i < N; ++i) {
-                    if (i >= p.n) break;
+                    const size_t row = static_cast<size_t>(tok0 + i);
                     const float2 v2 = unpack2(acc[i / 2]);
                     const float v = (i & 1 ? v2.y : v2.x) + bias;
-                    if (swiglu) {
+                    if (i >= rows) {
+                    } else if (swiglu) {
                         const float c = __shfl_xor_sync(0xffffffffu, v, 1);
-                        if (!(lane & 1) && j < p.m) y[static_cast<size_t>(i) * (p.m >> 1) + (j >> 1)] = from_float<T>(silu_fast(v) * c);
+                        if (!(lane & 1) && j < p.m) y[row * (p.m >> 1) + (j >> 1)] = from_float<T>(silu_fast(v) * c);
                     } else if (j < p.m) {
-                        put(y + static_cast<size_t>(i) * p.m + j, v, p.mode);
+                        put(y + row * p.m + j, v, p.mode);
                     }
                 }
             } else {
@@ -772,7 +716,7 @@ __global__ void __launch_bounds__(Few<N>::kThreads, 2)
 #pragma unroll
                 for (int i = 0; i < N; ++i) {
                     const float2 v2 = unpack2(acc[i / 2]);
-                    if (i < p.n) part[i * 128 + 32 * q + lane] = i & 1 ? v2.y : v2.x;
+                    if (i < rows) part[i * 128 + 32 * q + lane] = i & 1 ? v2.y : v2.x;
                 }
             }
         }
@@ -783,10 +727,11 @@ __global__ void __launch_bounds__(Few<N>::kThreads, 2)
         cluster_sync();
         // A cluster has one tile; this CTA finishes its share of the (token, 4 features) pieces.
         const uint32_t part = smem_u32(ring);
-        const int pieces = p.n * 32, e1 = static_cast<int>(static_cast<long long>(rank + 1) * pieces / p.split);
+        const int tok0 = unit % p.tiles_n * N, tm = unit / p.tiles_n;
+        const int pieces = min(N, p.n - tok0) * 32, e1 = static_cast<int>(static_cast<long long>(rank + 1) * pieces / p.split);
         T* y = static_cast<T*>(p.y);
         for (int e = static_cast<int>(static_cast<long long>(rank) * pieces / p.split) + threadIdx.x; e < e1; e += F::kThreads) {
-            const int tok = e >> 5, j = unit * 128 + (e & 31) * 4;
+            const int tok = tok0 + (e >> 5), j = tm * 128 + (e & 31) * 4;
             float4 v[kMaxSplit];
 #pragma unroll
             for (int k = 0; k < kMaxSplit; ++k) {
@@ -953,28 +898,65 @@ constexpr int kFewTokens = 64;  // most tokens of the kernel with features on th
 
 int cdiv(long long a, long long b) { return static_cast<int>((a + b - 1) / b); }
 
+// Clusters of `split` CTAs that the GPU runs at once with a CTA an SM (asked once a size).
+template <typename Kernel>
+int clusters_at_once(Kernel kernel, std::atomic<int>& known, int split, int threads) {
+    int n = known.load(std::memory_order_relaxed);
+    if (n) return n;
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(static_cast<unsigned>(split));
+    cfg.blockDim = dim3(static_cast<unsigned>(threads));
+    cfg.dynamicSmemBytes = kSmemLimit;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = static_cast<unsigned>(split);
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemLimit) != cudaSuccess ||
+        cudaOccupancyMaxActiveClusters(&n, kernel, &cfg) != cudaSuccess || n <= 0) {
+        cudaGetLastError();
+        return 0;
+    }
+    known.store(n, std::memory_order_relaxed);
+    return n;
+}
+
+// K split over how many CTAs: as many as run at once, powers of two.
 template <int N, typename T>
-cudaError_t launch_few_tokens(LinearParams& p, const uint8_t* xq, size_t ldx, const uint8_t* wq, size_t ldw, int k,
-                              int num_sms, cudaStream_t s) {
+int few_split(long long tiles, int blocks, int num_sms) {
+    static std::atomic<int> known[4];  // clusters of 2, 4, 8
+    int split = 1;
+    for (int i = 0, s = 2; s <= kMaxSplit && s <= blocks; ++i, s *= 2) {
+        // two CTAs an SM (fewer stages, see below) leave room to place the clusters of one wave of CTAs
+        const bool fits = Few<N>::kCtas > 1 ? tiles * s <= num_sms
+                                            : tiles <= clusters_at_once(linear_fp8_few_kernel<N, T>, known[i], s, Few<N>::kThreads);
+        if (!fits) break;
+        split = s;
+    }
+    return split;
+}
+
+template <int N, typename T>
+cudaError_t launch_features_on_lanes(LinearParams& p, const uint8_t* xq, size_t ldx, const uint8_t* wq, size_t ldw, int k,
+                                     int num_sms, cudaStream_t s) {
     using F = Few<N>;
-    p.tiles_n = 1;
+    p.tiles_n = cdiv(p.n, N);
     p.tiles_m = cdiv(p.m, 128);
-    p.x_rows = N;
-    p.stage_bytes = F::kStage;
+    const long long tiles = static_cast<long long>(p.tiles_n) * p.tiles_m;
     p.stages = std::min(kMaxStages, (kSmemLimit - 1024 - kBarBytes - F::kScaleBytes) / F::kStage);
-    p.split = 1;
-    while (p.split < kMaxSplit && static_cast<long long>(p.tiles_m) * p.split * 2 <= num_sms && p.split * 2 <= p.blocks)
-        p.split *= 2;
+    p.split = few_split<N, T>(tiles, p.blocks, num_sms);
     // A CTA of a split tile has few K-blocks and takes no more stages than those: several share an SM, so that the
-    // clusters run at once (36 clusters of 4 with an SM a CTA did not: 8.2 us where one wave takes half of that).
+    // clusters run at once (36 clusters of 4 with an SM a CTA did not: 8.2 us where one wave takes 5.7).
     if (p.split > 1)
-        p.stages = std::min(p.stages, std::max(cdiv(p.blocks, p.split), cdiv(static_cast<long long>(p.n) * 512, F::kStage)));
+        p.stages = std::min(p.stages, std::max(cdiv(p.blocks, p.split),
+                                               cdiv(static_cast<long long>(std::min(p.n, N)) * 512, F::kStage)));
     CUtensorMap mx, mw;
     cudaError_t e = make_byte_map(&mx, xq, p.n, k, ldx, N);
     if (e == cudaSuccess) e = make_byte_map(&mw, wq, p.m, k, ldw, 128);
     if (e != cudaSuccess) return e;
     static std::atomic<unsigned long long> allowed{0};
-    const int grid = p.split > 1 ? p.tiles_m * p.split : std::min(p.tiles_m, num_sms);
+    const int grid = static_cast<int>(p.split > 1 ? tiles * p.split : std::min<long long>(tiles, num_sms));
     return launch_linear(linear_fp8_few_kernel<N, T>, allowed, mx, mw, p, grid, F::kThreads, p.split,
                          p.stages * F::kStage + F::kScaleBytes + kBarBytes + 1024, s);
 }
@@ -990,34 +972,27 @@ cudaError_t launch_tokens(LinearParams& p, const uint8_t* xq, size_t ldx, const 
         const StreamParams sp{xq, wq, ldx, ldw, p.xs, p.ws, p.bias, p.y, p.mode, n, m, k, p.blocks};
         return launch_stream<T>(sp, num_sms, s);
     }
-    if (n <= 16) return launch_few_tokens<16, T>(p, xq, ldx, wq, ldw, k, num_sms, s);
-    if (n <= 32) return launch_few_tokens<32, T>(p, xq, ldx, wq, ldw, k, num_sms, s);
-    if (n <= kFewTokens) return launch_few_tokens<64, T>(p, xq, ldx, wq, ldw, k, num_sms, s);
+    if (n <= 16) return launch_features_on_lanes<16, T>(p, xq, ldx, wq, ldw, k, num_sms, s);
+    if (n <= 32) return launch_features_on_lanes<32, T>(p, xq, ldx, wq, ldw, k, num_sms, s);
+    if (n <= 64) return launch_features_on_lanes<64, T>(p, xq, ldx, wq, ldw, k, num_sms, s);
     // Rounds of K-blocks either tiling takes: a K-block costs about the same
-    // time in both (operands from L2), a pair's covers four times the outputs.
+    // time in both, a pair's covers four times the outputs.
     const long long t1 = static_cast<long long>(cdiv(n, 128)) * cdiv(m, 128);
     const long long t2 = static_cast<long long>(cdiv(n, 256)) * cdiv(m, 256);
     if (t1 > 0x3fffffffll) return cudaErrorInvalidValue;
-    int split = 1;
-    while (split < kMaxSplit && t1 * split * 2 <= num_sms && split * 2 <= p.blocks) split *= 2;
+    const int split = few_split<128, T>(t1, p.blocks, num_sms);
     const long long rounds1 = static_cast<long long>(cdiv(t1 * split, num_sms)) * cdiv(p.blocks, split);
     const long long rounds2 = static_cast<long long>(cdiv(t2, num_sms / 2)) * p.blocks;
-    const bool pair = n > 128 && rounds2 < rounds1;
-    p.split = pair ? 1 : split;
-    p.tiles_n = cdiv(n, pair ? 256 : 128);
-    p.tiles_m = cdiv(m, pair ? 256 : 128);
-    p.x_rows = pair || n >= kRows ? kRows : cdiv(n, 8) * 8;
-    p.stage_bytes = p.x_rows * kFp8Block + kOpBytes;
-    const int room = kSmemLimit - 1024 - kBarBytes - (pair ? Tile<2>::kStoreBytes : Tile<1>::kStoreBytes);
-    p.stages = std::min(kMaxStages, room / p.stage_bytes);
+    if (n <= 128 || rounds1 <= rounds2) return launch_features_on_lanes<128, T>(p, xq, ldx, wq, ldw, k, num_sms, s);
+    p.tiles_n = cdiv(n, 256);
+    p.tiles_m = cdiv(m, 256);
+    p.split = 1;
+    p.stages = std::min(kMaxStages, (kSmemLimit - 1024 - kBarBytes - Pair::kStoreBytes) / Pair::kStage);
     CUtensorMap mx, mw;
-    cudaError_t e = make_byte_map(&mx, xq, n, k, ldx, p.x_rows);
+    cudaError_t e = make_byte_map(&mx, xq, n, k, ldx, 128);
     if (e == cudaSuccess) e = make_byte_map(&mw, wq, m, k, ldw, 128);
     if (e != cudaSuccess) return e;
-    const long long tiles = static_cast<long long>(p.tiles_n) * p.tiles_m;
-    const int grid = pair ? 2 * static_cast<int>(std::min<long long>(tiles, num_sms / 2))
-                          : p.split * static_cast<int>(p.split > 1 ? tiles : std::min<long long>(tiles, num_sms));
-    return pair ? launch_tiled<2, T>(mx, mw, p, grid, s) : launch_tiled<1, T>(mx, mw, p, grid, s);
+    return launch_pairs<T>(mx, mw, p, 2 * static_cast<int>(std::min<long long>(t2, num_sms / 2)), s);
 }
 
 }  // namespace
