@@ -245,7 +245,8 @@ def linear_reference(torch, mode, x, xs, w, ws, bias, y0):
 
 LINEAR_SHAPES = [(1, 2, 1), (1, 130, 16), (2, 128, 128), (8, 576, 192), (17, 200, 300), (33, 384, 1536), (64, 256, 513),
                  (65, 1000, 257), (130, 258, 129), (300, 514, 1000), (257, 512, 2048), (1, 1030, 4096), (700, 1290, 640),
-                 (3, 20010, 130), (1100, 2602, 200), (2100, 2706, 257)]
+                 (3, 20010, 130), (1100, 2602, 200), (2100, 2706, 257), (1090, 2608, 640), (1500, 2336, 1050),
+                 (100, 1000, 513), (128, 770, 256)]
 
 
 @pytest.mark.parametrize("dtype", [0, 1, 2], ids=["fp32", "bf16", "fp16"])

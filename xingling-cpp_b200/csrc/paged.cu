@@ -22,36 +22,50 @@ __device__ __forceinline__ void rotate(float& a, float& b, float2 cs) {
 }
 
 // 16 elements a thread: of a key 8 pairs (j, j + d/2), of a value 16 in a row.
+// A copy, bound by its bytes; a CTA takes whole rows (kAppendThreads threads
+// over them), so that no index needs a 64-bit division.
+constexpr int kAppendThreads = 256;
 template <typename T, typename C>
-__global__ void __launch_bounds__(256) kv_append_paged_kernel(const PagedCache pc, const T* __restrict__ qkv,
-                                                              const float2* __restrict__ rope, int rope_len,
-                                                              const int* __restrict__ row_seq,
-                                                              const int* __restrict__ row_pos, int rows, int heads) {
-    const int d = pc.head_dim, per_head = d / 16, per_side = pc.kv_heads * per_head;
-    const long long id = static_cast<long long>(blockIdx.x) * 256 + threadIdx.x;
-    const int row = static_cast<int>(id / (2 * per_side));
-    if (row >= rows) return;
-    const int rest = static_cast<int>(id - static_cast<long long>(row) * (2 * per_side));
-    const bool value = rest >= per_side;
-    const int h = (value ? rest - per_side : rest) / per_head, part = (value ? rest - per_side : rest) % per_head;
-    const int seq = row_seq[row], pos = row_pos[row];
-    if (seq < 0 || seq >= pc.batch || !paged_pos_ok(pos, pc.max_pages, pc.page_size, rope ? rope_len : 0)) return;
-    const int page = pc.page_table[static_cast<int64_t>(seq) * pc.max_pages + pos / pc.page_size];
-    if (!paged_valid(page, pc.num_pages)) return;
-    const int64_t at = paged_base(page, h, pc.kv_heads, pc.page_size, d) + static_cast<int64_t>(pos % pc.page_size) * d;
-    const T* src = qkv + static_cast<int64_t>(row) * (heads + 2 * pc.kv_heads) * d +
-                   static_cast<int64_t>(heads + (value ? pc.kv_heads : 0) + h) * d;
-    const int e0 = value ? part * 16 : part * 8, e1 = value ? e0 + 8 : e0 + d / 2;
-    float a[8], b[8];
-    load8(src + e0, a);
-    load8(src + e1, b);
-    if (!value && rope) {
+__global__ void __launch_bounds__(kAppendThreads) kv_append_paged_kernel(const PagedCache pc, const T* __restrict__ qkv,
+                                                                         const float2* __restrict__ rope, int rope_len,
+                                                                         const int* __restrict__ row_seq,
+                                                                         const int* __restrict__ row_pos, int rows,
+                                                                         int heads, int rows_per_cta, FastDiv items_div,
+                                                                         FastDiv page_div) {
+    const int d = pc.head_dim, per_head = d / 16, per_side = pc.kv_heads * per_head, items = 2 * per_side;
+    for (int i = threadIdx.x; i < rows_per_cta * items; i += kAppendThreads) {
+        const int in = static_cast<int>(items_div.div(i)), rest = i - in * items;
+        const long long r = static_cast<long long>(blockIdx.x) * rows_per_cta + in;
+        if (r >= rows) return;
+        const int row = static_cast<int>(r);
+        const bool value = rest >= per_side;
+        const int of = value ? rest - per_side : rest, h = d == 64 ? of >> 2 : of >> 3, part = of & (per_head - 1);
+        const int seq = row_seq[row], pos = row_pos[row];
+        // the row's elements are on their way while its page is looked up
+        const T* src = qkv + static_cast<int64_t>(row) * (heads + 2 * pc.kv_heads) * d +
+                       static_cast<int64_t>(heads + (value ? pc.kv_heads : 0) + h) * d;
+        const int e0 = value ? part * 16 : part * 8, e1 = value ? e0 + 8 : e0 + d / 2;
+        float a[8], b[8];
+        load8(src + e0, a);
+        load8(src + e1, b);
+        if (seq < 0 || seq >= pc.batch || !paged_pos_ok(pos, pc.max_pages, pc.page_size, rope ? rope_len : 0)) continue;
+        const int n = static_cast<int>(page_div.div(pos));
+        const int page = pc.page_table[static_cast<int64_t>(seq) * pc.max_pages + n];
+        if (!paged_valid(page, pc.num_pages)) continue;
+        const int64_t at = paged_base(page, h, pc.kv_heads, pc.page_size, d) + static_cast<int64_t>(pos - n * pc.page_size) * d;
+        if (!value && rope) {
+            const float4* cs = reinterpret_cast<const float4*>(rope + static_cast<int64_t>(pos) * (d / 2) + e0);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) rotate(a[i], b[i], rope[static_cast<int64_t>(pos) * (d / 2) + e0 + i]);
+            for (int k = 0; k < 8; k += 2) {
+                const float4 x = cs[k / 2];
+                rotate(a[k], b[k], make_float2(x.x, x.y));
+                rotate(a[k + 1], b[k + 1], make_float2(x.z, x.w));
+            }
+        }
+        C* dst = static_cast<C*>(value ? pc.v : pc.k) + at;
+        store8(dst + e0, a);
+        store8(dst + e1, b);
     }
-    C* dst = static_cast<C*>(value ? pc.v : pc.k) + at;
-    store8(dst + e0, a);
-    store8(dst + e1, b);
 }
 
 // ---- attention of one new token a sequence ------------------------------------------------------------------------
@@ -702,12 +716,13 @@ __global__ void __launch_bounds__(128, (AttnShape<C, D, WIDE>::kCtas)) attn_deco
 template <typename T, typename C>
 cudaError_t append_typed(const PagedCache& pc, const void* qkv, const float* rope, int rope_len, const int* row_seq,
                          const int* row_pos, int rows, int heads, cudaStream_t s) {
-    const long long items = static_cast<long long>(rows) * pc.kv_heads * (pc.head_dim / 8);
-    const long long ctas = (items + 255) / 256;
-    if (ctas > 0x7fffffffll) return cudaErrorInvalidValue;
+    const long long items = static_cast<long long>(pc.kv_heads) * (pc.head_dim / 8);
+    if (items > 0x3fffffff) return cudaErrorInvalidValue;
+    const int each = static_cast<int>(items), per_cta = std::max(1, kAppendThreads / each);
     count_launch();
-    kv_append_paged_kernel<T, C><<<static_cast<int>(ctas), 256, 0, s>>>(
-        pc, static_cast<const T*>(qkv), reinterpret_cast<const float2*>(rope), rope_len, row_seq, row_pos, rows, heads);
+    kv_append_paged_kernel<T, C><<<(rows - 1) / per_cta + 1, kAppendThreads, 0, s>>>(
+        pc, static_cast<const T*>(qkv), reinterpret_cast<const float2*>(rope), rope_len, row_seq, row_pos, rows, heads,
+        per_cta, FastDiv(static_cast<uint32_t>(each)), FastDiv(static_cast<uint32_t>(pc.page_size)));
     return cudaGetLastError();
 }
 
