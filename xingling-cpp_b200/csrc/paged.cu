@@ -193,8 +193,15 @@ __device__ __forceinline__ void split16(float a, float b, uint32_t& hi, uint32_t
     hi = pack16(ha, hb, C{});
     lo = pack16(a - ha, b - hb, C{});
 }
-__device__ __forceinline__ uint32_t tf32_lo(uint32_t v) {
-    return __float_as_uint(__uint_as_float(v) - __uint_as_float(v & 0xffffe000u));
+// v = hi + lo for TF32 products: hi to nearest, so that what lo loses (it is
+// cut to 11 bits) has no sign of its own.
+__device__ __forceinline__ uint32_t tf32_hi(uint32_t v) {
+    uint32_t r;
+    asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(r) : "f"(__uint_as_float(v)));
+    return r;
+}
+__device__ __forceinline__ uint32_t tf32_lo(uint32_t v, uint32_t hi) {
+    return __float_as_uint(__uint_as_float(v) - __uint_as_float(hi));
 }
 
 __device__ __forceinline__ void mma16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1, __nv_bfloat16) {
@@ -450,8 +457,9 @@ __global__ void __launch_bounds__(128, (AttnShape<C, D, WIDE>::kCtas)) attn_deco
             if constexpr (S::k32) {
                 const uint32_t a0 = __float_as_uint(qa[n][0]), a1 = __float_as_uint(qa[n][1]);
                 const uint32_t b0 = __float_as_uint(qb[n][0]), b1 = __float_as_uint(qb[n][1]);
-                *fa = make_uint4(a0, a1, tf32_lo(a0), tf32_lo(a1));
-                *fb = make_uint4(b0, b1, tf32_lo(b0), tf32_lo(b1));
+                const uint32_t ha0 = tf32_hi(a0), ha1 = tf32_hi(a1), hb0 = tf32_hi(b0), hb1 = tf32_hi(b1);
+                *fa = make_uint4(ha0, ha1, tf32_lo(a0, ha0), tf32_lo(a1, ha1));
+                *fb = make_uint4(hb0, hb1, tf32_lo(b0, hb0), tf32_lo(b1, hb1));
             } else {
                 uint4 o;
                 split16<C>(qa[n][0] * down, qa[n][1] * down, o.x, o.z);
@@ -497,11 +505,13 @@ __global__ void __launch_bounds__(128, (AttnShape<C, D, WIDE>::kCtas)) attn_deco
             const int x0 = c * kChunk + warp * kTile;
             if (x0 > pos) break;  // only the last chunk has tiles past the end
             const uint32_t next = find_rows(c + 1);
-            float s[S::kHalves][4], more[S::kHalves][4];
+            // The MMA cuts its sums instead of rounding them, so long sums are kept out of it: the 8 or 16 large products
+            // of an fp32 cache in two halves, added here; the outputs tile by tile.
+            float s[S::kHalves][4], also[S::kHalves][4], more[S::kHalves][4];
 #pragma unroll
             for (int h = 0; h < S::kHalves; ++h)
 #pragma unroll
-                for (int j = 0; j < 4; ++j) s[h][j] = more[h][j] = 0.0f;
+                for (int j = 0; j < 4; ++j) s[h][j] = also[h][j] = more[h][j] = 0.0f;
 #pragma unroll
             for (int i = 0; i < S::kSteps; ++i) {
                 const int w = (i & 1) * 2;
@@ -509,13 +519,16 @@ __global__ void __launch_bounds__(128, (AttnShape<C, D, WIDE>::kCtas)) attn_deco
 #pragma unroll
                 for (int h = 0; h < S::kHalves; ++h) {
                     const uint4 q = load_shared(frag + (i * S::kHalves + h) * 32 + lane);
+                    float(&large)[4] = S::k32 && (i & 1) ? also[h] : s[h];
                     if constexpr (S::k32) {
-                        const uint32_t lo[4] = {tf32_lo(a[0]), tf32_lo(a[1]), tf32_lo(a[2]), tf32_lo(a[3])};
-                        mma_tf32(s[h], a, q.x, q.y);
-                        mma_tf32(more[h], a, q.z, q.w);
+                        const uint32_t hi[4] = {tf32_hi(a[0]), tf32_hi(a[1]), tf32_hi(a[2]), tf32_hi(a[3])};
+                        const uint32_t lo[4] = {tf32_lo(a[0], hi[0]), tf32_lo(a[1], hi[1]), tf32_lo(a[2], hi[2]),
+                                                tf32_lo(a[3], hi[3])};
+                        mma_tf32(large, hi, q.x, q.y);
+                        mma_tf32(more[h], hi, q.z, q.w);
                         mma_tf32(more[h], lo, q.x, q.y);
                     } else {
-                        mma16(s[h], a, q.x, q.y, C{});
+                        mma16(large, a, q.x, q.y, C{});
                         mma16(more[h], a, q.z, q.w, C{});
                     }
                 }
@@ -526,7 +539,7 @@ __global__ void __launch_bounds__(128, (AttnShape<C, D, WIDE>::kCtas)) attn_deco
 #pragma unroll
             for (int h = 0; h < S::kHalves; ++h) {
 #pragma unroll
-                for (int j = 0; j < 4; ++j) s[h][j] = (s[h][j] + more[h][j]) * back[h][j & 1];
+                for (int j = 0; j < 4; ++j) s[h][j] = (s[h][j] + also[h][j] + more[h][j]) * back[h][j & 1];
                 if (x0 + kTile > pos + 1) {
 #pragma unroll
                     for (int j = 0; j < 4; ++j)
@@ -564,9 +577,9 @@ __global__ void __launch_bounds__(128, (AttnShape<C, D, WIDE>::kCtas)) attn_deco
                     if constexpr (S::k32) {
                         const uint32_t x = __float_as_uint(s[h][2 * n]), y = __float_as_uint(s[h][2 * n + 1]);
                         const uint32_t up = transpose8(__byte_perm(x, y, 0x7632)), down = transpose8(__byte_perm(x, y, 0x5410));
-                        wh[h][2 * n] = __byte_perm(down, up, 0x5410);
-                        wh[h][2 * n + 1] = __byte_perm(down, up, 0x7632);
-                        wl[h][2 * n] = tf32_lo(wh[h][2 * n]), wl[h][2 * n + 1] = tf32_lo(wh[h][2 * n + 1]);
+                        const uint32_t w0 = __byte_perm(down, up, 0x5410), w1 = __byte_perm(down, up, 0x7632);
+                        wh[h][2 * n] = tf32_hi(w0), wh[h][2 * n + 1] = tf32_hi(w1);
+                        wl[h][2 * n] = tf32_lo(w0, wh[h][2 * n]), wl[h][2 * n + 1] = tf32_lo(w1, wh[h][2 * n + 1]);
                     } else {
                         uint32_t hi, lo;
                         split16<C>(s[h][2 * n], s[h][2 * n + 1], hi, lo);
@@ -576,18 +589,25 @@ __global__ void __launch_bounds__(128, (AttnShape<C, D, WIDE>::kCtas)) attn_deco
 #pragma unroll
             for (int i = 0; i < D / 16; ++i) {
                 const int ch = i / (S::kVec / 2), e = i % (S::kVec / 2);
+                float o[S::kHalves][4];
+#pragma unroll
+                for (int h = 0; h < S::kHalves; ++h)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) o[h][j] = 0.0f;
                 if constexpr (S::k32) {
                     // position 2t is the MMA's k = t, 2t + 1 its k = t + 4; columns 2e and 2e + 1 its rows g and g + 8
 #pragma unroll
                     for (int n = 0; n < 2; ++n) {
                         const uint32_t a[4] = {word(vr[2 * n][ch], 2 * e), word(vr[2 * n][ch], 2 * e + 1),
                                                word(vr[2 * n + 1][ch], 2 * e), word(vr[2 * n + 1][ch], 2 * e + 1)};
-                        const uint32_t lo[4] = {tf32_lo(a[0]), tf32_lo(a[1]), tf32_lo(a[2]), tf32_lo(a[3])};
+                        const uint32_t hi[4] = {tf32_hi(a[0]), tf32_hi(a[1]), tf32_hi(a[2]), tf32_hi(a[3])};
+                        const uint32_t lo[4] = {tf32_lo(a[0], hi[0]), tf32_lo(a[1], hi[1]), tf32_lo(a[2], hi[2]),
+                                                tf32_lo(a[3], hi[3])};
 #pragma unroll
                         for (int h = 0; h < S::kHalves; ++h) {
-                            mma_tf32(acc[h][i], a, wh[h][2 * n], wh[h][2 * n + 1]);
-                            mma_tf32(acc[h][i], a, wl[h][2 * n], wl[h][2 * n + 1]);
-                            mma_tf32(acc[h][i], lo, wh[h][2 * n], wh[h][2 * n + 1]);
+                            mma_tf32(o[h], lo, wh[h][2 * n], wh[h][2 * n + 1]);
+                            mma_tf32(o[h], hi, wl[h][2 * n], wl[h][2 * n + 1]);
+                            mma_tf32(o[h], hi, wh[h][2 * n], wh[h][2 * n + 1]);
                         }
                     }
                 } else {
@@ -596,10 +616,14 @@ __global__ void __launch_bounds__(128, (AttnShape<C, D, WIDE>::kCtas)) attn_deco
                                            __byte_perm(z, u, 0x7632)};
 #pragma unroll
                     for (int h = 0; h < S::kHalves; ++h) {
-                        mma16(acc[h][i], a, wh[h][0], wh[h][1], C{});
-                        mma16(acc[h][i], a, wl[h][0], wl[h][1], C{});
+                        mma16(o[h], a, wl[h][0], wl[h][1], C{});
+                        mma16(o[h], a, wh[h][0], wh[h][1], C{});
                     }
                 }
+#pragma unroll
+                for (int h = 0; h < S::kHalves; ++h)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) acc[h][i][j] += o[h][j];
             }
             load_v(next);
         }
