@@ -24,6 +24,16 @@ __device__ __forceinline__ __nv_bfloat16 from_float<__nv_bfloat16>(float v) { re
 template <>
 __device__ __forceinline__ __half from_float<__half>(float v) { return __float2half_rn(v); }
 
+// Two floats to the low and high half of a word.
+__device__ __forceinline__ uint32_t pack_pair(float lo, float hi, __nv_bfloat16) {
+    const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&v);
+}
+__device__ __forceinline__ uint32_t pack_pair(float lo, float hi, __half) {
+    const __half2 v = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&v);
+}
+
 // 8 consecutive elements of a 16-byte aligned address, as floats.
 template <typename T>
 __device__ __forceinline__ void load8(const T* p, float (&v)[8]) {
@@ -79,6 +89,27 @@ __device__ __forceinline__ void to_floats(const Raw8<T>& r, float (&v)[8]) {
     const T* e = reinterpret_cast<const T*>(&r);
 #pragma unroll
     for (int i = 0; i < 8; ++i) v[i] = to_float(e[i]);
+}
+
+// 8 floats rounded to T, as they lie in memory.
+template <typename T>
+__device__ __forceinline__ Raw8<T> round_raw8(const float (&v)[8]) {
+    Raw8<T> r;
+    if constexpr (sizeof(T) == 4) {
+        float* e = reinterpret_cast<float*>(&r);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) e[i] = v[i];
+    } else {
+        uint32_t* w = reinterpret_cast<uint32_t*>(&r);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) w[i] = pack_pair(v[2 * i], v[2 * i + 1], T{});
+    }
+    return r;
+}
+template <typename T>
+__device__ __forceinline__ void store_raw8(T* p, const Raw8<T>& r) {
+#pragma unroll
+    for (int i = 0; i < static_cast<int>(sizeof(T) / 2); ++i) reinterpret_cast<uint4*>(p)[i] = r.w[i];
 }
 
 // Two floats to two e4m3 bytes (the first in the low byte), to nearest, ties to even; NaN stays NaN.

@@ -178,20 +178,12 @@ __device__ __forceinline__ int row_exponent(uint32_t bits) {
     return bits == 0u || bits >= 0x7f800000u ? 0 : max(-120, min(120, e));
 }
 
-__device__ __forceinline__ uint32_t pack16(float lo, float hi, __nv_bfloat16) {
-    const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
-    return *reinterpret_cast<const uint32_t*>(&v);
-}
-__device__ __forceinline__ uint32_t pack16(float lo, float hi, __half) {
-    const __half2 v = __floats2half2_rn(lo, hi);
-    return *reinterpret_cast<const uint32_t*>(&v);
-}
 // Two values as a pair of 16-bit halves: v = hi + lo up to 2^-17 (bf16) or 2^-22 (fp16) of it.
 template <typename C>
 __device__ __forceinline__ void split16(float a, float b, uint32_t& hi, uint32_t& lo) {
     const float ha = to_float(from_float<C>(a)), hb = to_float(from_float<C>(b));
-    hi = pack16(ha, hb, C{});
-    lo = pack16(a - ha, b - hb, C{});
+    hi = pack_pair(ha, hb, C{});
+    lo = pack_pair(a - ha, b - hb, C{});
 }
 // v = hi + lo for TF32 products: hi to nearest, so that what lo loses (it is
 // cut to 11 bits) has no sign of its own.

@@ -184,7 +184,7 @@ __device__ __forceinline__ double inverse_root(double v) {
 // of a group is taken with the remainder of its fp32 product (rounding keeps
 // the order), so that a group's scale is the rounded exact one.
 template <typename T, int CHUNKS, int THREADS, bool VEC>
-__global__ void __launch_bounds__(THREADS) add_rmsnorm_fp8_kernel(const T* __restrict__ delta, const T* residual, T* sum,
+__global__ void __launch_bounds__(THREADS, THREADS == 256 ? 3 : 1) add_rmsnorm_fp8_kernel(const T* __restrict__ delta, const T* residual, T* sum,
                                                                   const float* __restrict__ gamma,
                                                                   uint8_t* __restrict__ q, size_t ldq,
                                                                   float* __restrict__ scale, int k) {
@@ -213,10 +213,15 @@ __global__ void __launch_bounds__(THREADS) add_rmsnorm_fp8_kernel(const T* __res
             float d[8];
             to_floats(raw_d[j], d);
 #pragma unroll
-            for (int i = 0; i < 8; ++i) r[j][i] = to_float(from_float<T>(r[j][i] + d[i]));
-            if (VEC) {
-                if (live) store8(sum + at, r[j]);
+            for (int i = 0; i < 8; ++i) r[j][i] += d[i];
+            if constexpr (sizeof(T) == 2) {
+                const Raw8<T> rounded = round_raw8<T>(r[j]);
+                to_floats(rounded, r[j]);
+                if (VEC && live) store_raw8(sum + at, rounded);
             } else {
+                if (VEC && live) store8(sum + at, r[j]);
+            }
+            if (!VEC) {
 #pragma unroll
                 for (int i = 0; i < 8; ++i)
                     if (i < live) sum[at + i] = from_float<T>(r[j][i]);
@@ -244,15 +249,16 @@ __global__ void __launch_bounds__(THREADS) add_rmsnorm_fp8_kernel(const T* __res
         const int live = max(0, min(8, k - c));
         float w[8], p[8];
         to_floats(load_raw8<VEC>(gamma + (live ? c : 0), live), w);
-        float own = -1.0f, own_r = 0.0f, own_w = 0.0f;  // the lane's largest product and its factors
-        bool nan = false;
+        float own = 0.0f, own_r = 0.0f, own_w = 0.0f;  // the lane's largest product (NaN if there is one), its factors
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
             p[i] = r[j][i] * w[i];
-            nan |= p[i] != p[i];
-            if (fabsf(p[i]) > own) own = fabsf(p[i]), own_r = r[j][i], own_w = w[i];
+            const float size = fabsf(p[i]);
+            const bool up = size > own;
+            own_r = up ? r[j][i] : own_r, own_w = up ? w[i] : own_w;
+            asm("max.NaN.f32 %0, %0, %1;" : "+f"(own) : "f"(size));
         }
-        const uint32_t mine = nan ? 0x7fffffffu : __float_as_uint(own);
+        const uint32_t mine = __float_as_uint(own);
         uint32_t a = mine;
 #pragma unroll
         for (int o = kLanesPerGroup / 2; o; o >>= 1) a = umax(a, __shfl_xor_sync(0xffffffffu, a, o));
