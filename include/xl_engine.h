@@ -401,7 +401,7 @@ XL_API int xl_op_linear_fp8(int mode, int dtype, const uint8_t* xq, size_t ldx, 
 
 /* A paged cache: pools k and v [num_pages][kv_heads][page_size][head_dim] of
  * dtype; page_table [batch][max_pages] (device ints) names the pages of each
- * sequence in order.  head_dim 64 or 128; max_pages * page_size <= 2^31 - 1,
+ * sequence in order.  head_dim 64 or 128; max_pages * page_size <= 2^31 - 65536,
  * num_pages * kv_heads * page_size <= 2^32 - 2, batch * heads < 2^30.
  * Entries past the pages that a sequence's positions need are not read.
  * Sequences may share pages that are not written any more.  The struct itself
@@ -425,7 +425,8 @@ typedef struct xl_paged_kv {
  * angles rope[row_pos[i]] ([rope_len][head_dim / 2] pairs of cos and sin:
  * xl_rope_table for head_dim 64) or as it is where rope is NULL.  A row whose
  * sequence, position or page is out of range is skipped; positions past
- * rope_len are out of range.  Two rows for one position: either is stored. */
+ * rope_len are out of range.  No two rows may name one position (what is
+ * stored there is then a mixture of theirs). */
 XL_API int xl_op_kv_append_paged(const xl_paged_kv* cache, int dtype, const void* qkv, const float* rope, int rope_len,
                                  const int* row_seq, const int* row_pos, int rows, int heads, void* stream);
 

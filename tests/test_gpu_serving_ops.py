@@ -707,3 +707,151 @@ def test_layer_step(torch):
         y, tol = plain("w2", f8, fs, ffn)
         want = r.double() + y
         assert ((x2.cpu().double() - want).abs() <= tol + 4 * U * (want.abs() + tol)).all()
+
+
+# ---- far offsets, refusals that need a device, streams -----------------------------------------------------------------
+
+def test_quantize_and_linear_past_2g(torch):
+    """Matrices of more than 2^31 bytes and elements: their last rows."""
+    m, k = 140001, 16384
+    x = torch.empty((m, k), dtype=torch.bfloat16, device="cuda")
+    tail = torch.randn((300, k), generator=gen(torch, 1)).bfloat16()
+    x.zero_()
+    x[-300:] = tail.cuda()
+    q, s = torch.empty((m, k), dtype=torch.uint8, device="cuda"), torch.empty(((m + 127) // 128, k // 128), device="cuda")
+    X.check(X.lib().xl_op_quantize_fp8(1, X.ptr(x), k, X.ptr(q), k, X.ptr(s), m, k, 128, X.stream()))
+    torch.cuda.synchronize()
+    first = (m - 300 + 127) // 128 * 128  # the first whole block of rows in the tail
+    want_q, want_s = quantise(torch, tail[first - (m - 300):].double(), 128)
+    same(torch, s[first // 128:], want_s)
+    same(torch, q[first:].view(torch.float8_e4m3fn), want_q)
+    rows = torch.empty_like(q)
+    per_row = torch.empty((m, k // 128), device="cuda")
+    X.check(X.lib().xl_op_quantize_fp8(1, X.ptr(x), k, X.ptr(rows), k, X.ptr(per_row), m, k, 1, X.stream()))
+    torch.cuda.synchronize()
+    want_rq, want_rs = quantise(torch, tail[-3:].double(), 1)
+    same(torch, per_row[-3:], want_rs)
+    same(torch, rows[-3:].view(torch.float8_e4m3fn), want_rq)
+    for n in (2, 70):
+        (dx, xv) = random_fp8(torch, n, k, gen(torch, n))
+        xs = torch.rand((n, k // 128), generator=gen(torch, 9)) * 0.01
+        dxs = xs.cuda()
+        y = torch.empty((n, m), device="cuda")
+        X.check(X.lib().xl_op_linear_fp8(0, 0, X.ptr(dx), k, X.ptr(dxs), X.ptr(q), k, X.ptr(s), None, X.ptr(y), n, m, k,
+                                         X.stream()))
+        torch.cuda.synchronize()
+        want, bound = linear_reference(torch, 0, xv, xs, want_q, want_s.float(), None, None)
+        off = (y[:, first:].cpu().double() - want).abs() - bound - U * want.abs()
+        assert (off <= 0).all(), float(off.max())
+
+
+def test_attend_and_append_past_2g(torch):
+    """A pool of more than 2^31 elements: the pages at its end."""
+    kv, d, page, heads = 2, 128, 64, 8
+    pages = (1 << 31) // (kv * d * page) + 40
+    c = X.PagedKV()
+    k, v = (torch.empty((pages, kv, page, d), dtype=torch.float16, device="cuda") for _ in range(2))
+    ids = [pages - 1, pages - 30, pages - 7, pages - 2]
+    table = torch.tensor([ids], dtype=torch.int32)
+    dt = table.cuda()
+    c = X.PagedKV(k.data_ptr(), v.data_ptr(), dt.data_ptr(), 2, 1, kv, d, page, 4, pages)
+    n = 3 * page + 17
+    rope = rope_table(torch, n + 1, d)
+    dr = rope.cuda()
+    prompt = torch.randn((n, (heads + 2 * kv) * d), generator=gen(torch, 2))
+    dp, seq, at = prompt.cuda(), torch.zeros(n, dtype=torch.int32, device="cuda"), torch.arange(n, dtype=torch.int32, device="cuda")
+    X.check(X.lib().xl_op_kv_append_paged(C.byref(c), 0, X.ptr(dp), X.ptr(dr), n + 1, X.ptr(seq), X.ptr(at), n, heads, X.stream()))
+    p = Paged.__new__(Paged)
+    p.torch, p.page, p.kv, p.d, p.c, p.table = torch, page, kv, d, c, torch.tensor([[0, 1, 2, 3]], dtype=torch.int32)
+    qkv = torch.randn((1, (heads + 2 * kv) * d), generator=gen(torch, 3))
+    dq, pos, out = qkv.cuda(), torch.tensor([n], dtype=torch.int32, device="cuda"), torch.empty((1, heads * d), device="cuda")
+    attend(torch, p, 0, dq, dr, pos, out, heads, workspace(torch, c, heads))
+    torch.cuda.synchronize()
+    p.dk, p.dv = k[ids].contiguous(), v[ids].contiguous()  # the same pages under the numbers 0 .. 3
+    p.k = p.dk
+    split = prompt.view(n, heads + 2 * kv, d)
+    keys, values = p.rows(0, n)
+    assert torch.equal(values, split[:, heads + kv:].transpose(0, 1).half().double())
+    want = rotate(torch, split[:, heads:heads + kv], rope[:n, None]).transpose(0, 1)
+    assert ((keys - want).abs() <= half_step(torch, torch.float16) * want.abs() + 8 * U * 8).all()
+    check_attention(torch, p, qkv, rope, [n], out, heads)
+
+
+def test_host_memory_is_refused(torch):
+    """A pointer to pageable host memory ends in a status before anything is launched."""
+    host = torch.zeros(1 << 12)
+    q, s = torch.empty((4, 256), dtype=torch.uint8, device="cuda"), torch.empty((4, 2), device="cuda")
+    assert X.lib().xl_op_quantize_fp8(0, X.ptr(host) + -X.ptr(host) % 16, 256, X.ptr(q), 256, X.ptr(s), 4, 256, 1, X.stream()) == 1
+    assert b"current device" in X.lib().xl_last_error()
+
+
+def test_products_on_several_streams_at_once(torch):
+    """Calls of different shapes under way together (clusters that share SMs) give what each gives alone."""
+    cases = []
+    for i, (n, m, k) in enumerate([(8, 4608, 1536), (16, 1536, 4096), (32, 4608, 1536), (64, 1536, 4096), (100, 1536, 1536),
+                                   (300, 4608, 1536), (12, 512, 2048)]):
+        g = gen(torch, i)
+        (dx, x), (dw, w) = random_fp8(torch, n, k, g), random_fp8(torch, m, k, g)
+        xs, ws = torch.rand((n, k // 128), generator=g).cuda(), (torch.rand((m // 128, k // 128), generator=g) * 1e-3).cuda()
+        cases.append((n, m, k, dx, dw, xs, ws, torch.empty((n, m), device="cuda"), torch.cuda.Stream()))
+
+    def call(c, y, stream):
+        n, m, k, dx, dw, xs, ws = c[:7]
+        X.check(X.lib().xl_op_linear_fp8(0, 0, X.ptr(dx), dx.stride(0), X.ptr(xs), X.ptr(dw), dw.stride(0), X.ptr(ws), None,
+                                         X.ptr(y), n, m, k, C.c_void_p(stream.cuda_stream)))
+
+    torch.cuda.synchronize()
+    alone = []
+    for c in cases:
+        y = torch.empty_like(c[7])
+        call(c, y, torch.cuda.current_stream())
+        torch.cuda.synchronize()
+        alone.append(y)
+    for _ in range(20):
+        for c in cases:
+            call(c, c[7], c[8])
+    torch.cuda.synchronize()
+    for c, y in zip(cases, alone):
+        assert torch.equal(c[7], y), c[:3]
+
+
+def test_first_calls_inside_a_capture(torch):
+    """Each operator's first call of a process may be the captured one (kernels are loaded, limits raised on the way)."""
+    import os
+    import subprocess
+    import sys
+
+    code = r'''
+import ctypes as C, sys
+sys.path[:0] = ["tests", "xingling-cpp_b200"]
+import torch, xl_capi as X
+z = lambda *s, dt=torch.float32: torch.zeros(s, dtype=dt, device="cuda")
+side = torch.cuda.Stream(); st = C.c_void_p(side.cuda_stream)
+x, q, s = z(600, 512) + 1, z(600, 512, dt=torch.uint8), z(600, 4)
+w, ws = z(4096, 512, dt=torch.uint8) + 0x38, z(32, 4) + 1  # 0x38 is 1.0
+g, y = z(512) + 1, z(600, 4096)
+table, pos, seq = z(2, 4, dt=torch.int32), z(2, dt=torch.int32), z(2, dt=torch.int32)
+table[1] = 1
+k, v = z(2, 2, 16, 64), z(2, 2, 16, 64)
+qkv, out = z(2, (4 + 4) * 64) + 1, z(2, 256)
+c = X.PagedKV(k.data_ptr(), v.data_ptr(), table.data_ptr(), 0, 2, 2, 64, 16, 4, 2)
+wk = z(X.lib().xl_op_attn_decode_paged_workspace_bytes(C.byref(c), 4), dt=torch.uint8)
+torch.cuda.synchronize()
+graph = torch.cuda.CUDAGraph()
+L, P = X.lib(), X.ptr
+with torch.cuda.graph(graph, stream=side):
+    X.check(L.xl_op_quantize_fp8(0, P(x), 512, P(q), 512, P(s), 600, 512, 1, st))
+    X.check(L.xl_op_add_rmsnorm_fp8(0, None, P(x), None, P(g), P(q), 512, P(s), 600, 512, st))
+    for n in (8, 16, 64, 100, 600):
+        X.check(L.xl_op_linear_fp8(0, 0, P(q), 512, P(s), P(w), 512, P(ws), None, P(y), n, 4096, 512, st))
+    X.check(L.xl_op_kv_append_paged(C.byref(c), 0, P(qkv), None, 0, P(seq), P(pos), 2, 4, st))
+    X.check(L.xl_op_attn_decode_paged(C.byref(c), 0, P(qkv), None, 0, P(pos), P(out), 4, P(wk), wk.numel(), st))
+graph.replay()
+torch.cuda.synchronize()
+assert (y - 512).abs().max() < 1e-2, y
+assert (out == 1).all()
+print("captured")
+'''
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, cwd=root, timeout=300)
+    assert r.returncode == 0 and "captured" in r.stdout, r.stdout + r.stderr

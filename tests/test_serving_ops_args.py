@@ -64,7 +64,7 @@ CACHE_FAULTS = [
     (dict(k=None), "null"), (dict(v=None), "null"), (dict(page_table=None), "null"), (dict(dtype=4), "dtype"),
     (dict(batch=0), "positive"), (dict(kv_heads=0), "positive"), (dict(page_size=0), "positive"),
     (dict(max_pages=0), "positive"), (dict(num_pages=-2), "positive"), (dict(head_dim=96), "head_dim"),
-    (dict(kv_heads=3), "multiple"), (dict(page_size=1 << 16, max_pages=1 << 16), "2^31"),
+    (dict(kv_heads=3), "multiple"), (dict(page_size=1 << 16, max_pages=1 << 16), "2^31"), (dict(page_size=1 << 10, max_pages=(1 << 21) - 1), "2^31"),
     (dict(batch=1 << 30), "2^30"), (dict(k=P + 8), "aligned"), (dict(num_pages=1 << 30), "2^32"),
 ]
 

@@ -521,7 +521,7 @@ const char* paged_fault(const xl_paged_kv* c, int heads) {
         return "sizes must be positive";
     if (c->head_dim != 64 && c->head_dim != 128) return "head_dim must be 64 or 128";
     if (heads % c->kv_heads) return "heads must be a multiple of kv_heads";
-    if (static_cast<long long>(c->max_pages) * c->page_size > 0x7fffffffll) return "max_pages * page_size is over 2^31 - 1";
+    if (static_cast<long long>(c->max_pages) * c->page_size > 0x7fff0000ll) return "max_pages * page_size is over 2^31 - 65536";
     if (static_cast<double>(c->num_pages) * c->kv_heads * c->page_size > 4294967294.0)
         return "num_pages * kv_heads * page_size is over 2^32 - 2";
     if (static_cast<long long>(c->batch) * heads > 0x3fffffffll) return "batch * heads is over 2^30 - 1";

@@ -5,6 +5,7 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include "paged.h"
 #include "xl_kernels.h"
 
 namespace xl {
@@ -142,28 +143,5 @@ __device__ __forceinline__ bool near_border_small(float q) {
     const float m = fabsf(q) * 1024.0f, r = rintf(m);
     return m <= 16.5f && fabsf(m - r) < 4e-5f && (static_cast<int>(r) & 1);
 }
-
-// n / d for 0 <= n < 2^31 with a multiplication (Granlund and Montgomery,
-// "Division by invariant integers using multiplication", PLDI 1994): with
-// l = ceil(log2 d) and mul = floor(2^32 (2^l - d) / d) + 1 the quotient is
-// (hi + (n - hi) / 2) >> (l - 1), hi the high word of n * mul.
-struct FastDiv {
-    uint32_t d, mul, shift;
-    FastDiv() = default;
-    explicit FastDiv(uint32_t div) : d(div) {
-        uint32_t l = 0;
-        while ((1ull << l) < div) ++l;
-        mul = static_cast<uint32_t>(((1ull << 32) * ((1ull << l) - div)) / div + 1);
-        shift = l;
-    }
-    __host__ __device__ __forceinline__ uint32_t div(uint32_t n) const {
-#ifdef __CUDA_ARCH__
-        const uint32_t hi = __umulhi(n, mul);
-#else
-        const uint32_t hi = static_cast<uint32_t>((static_cast<uint64_t>(n) * mul) >> 32);
-#endif
-        return shift ? (hi + ((n - hi) >> 1)) >> (shift - 1) : n;
-    }
-};
 
 }  // namespace xl

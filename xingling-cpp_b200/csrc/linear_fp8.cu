@@ -957,8 +957,12 @@ cudaError_t launch_features_on_lanes(LinearParams& p, const uint8_t* xq, size_t 
     if (e != cudaSuccess) return e;
     static std::atomic<unsigned long long> allowed{0};
     const int grid = static_cast<int>(p.split > 1 ? tiles * p.split : std::min<long long>(tiles, num_sms));
+    // Shared memory in proportion to the TMEM columns, so that no mix of CTAs on an SM asks for more than its 512: a
+    // CTA that waits for columns while its cluster's others hold some could otherwise wait for a cluster that waits
+    // for it.  (An SM has 228 KB, each CTA 1 KB of its own.)
+    const int share = static_cast<int>(233472ll * F::kColumns / 512) - 1024;
     return launch_linear(linear_fp8_few_kernel<N, T>, allowed, mx, mw, p, grid, F::kThreads, p.split,
-                         p.stages * F::kStage + F::kScaleBytes + kBarBytes + 1024, s);
+                         std::max(share, p.stages * F::kStage + F::kScaleBytes + kBarBytes + 1024), s);
 }
 
 template <typename T>

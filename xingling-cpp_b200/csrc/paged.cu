@@ -99,13 +99,12 @@ __global__ void __launch_bounds__(kAppendThreads) kv_append_paged_kernel(const P
 // products of split operands.  Sums, maxima and the running output are fp32.
 
 constexpr int kAttnWarps = 4;
-constexpr int kAttnMaxCtas = 740;            // 148 SMs x 5
 constexpr int kAttnShort = 8;                // chunks a CTA up to which stretches keep to one pair
 constexpr int kAttnTries = 6;
 constexpr int kMergeAhead = 8;
 constexpr int kAttnRows = 16;                // most query heads of a pair
 constexpr size_t kAttnSlotFloats = kAttnRows * (128 + 2);
-constexpr size_t kAttnPartBytes = kAttnMaxCtas * 2 * kAttnSlotFloats * 4;  // two partials a CTA
+constexpr size_t kAttnPartBytes = kPagedMaxCtas * 2 * kAttnSlotFloats * 4;  // two partials a CTA
 constexpr int kTile = 16;                    // positions of a warp's tile
 constexpr int kChunk = kAttnWarps * kTile;
 constexpr float kLog2e = 1.4426950408889634f;
@@ -294,13 +293,9 @@ __global__ void __launch_bounds__(128, (AttnShape<C, D, WIDE>::kCtas)) attn_deco
     }
     const long long grid = min(static_cast<long long>(gridDim.x), all);  // a unit at least for every CTA that works
     if (blockIdx.x >= grid) return;
-    // (64-bit divisions take hundreds of clocks: 32 bits where they do)
-    const bool brief = all < (1ll << 31) / kAttnMaxCtas;
-    auto share = [&](unsigned i) {
-        return brief ? static_cast<long long>(i * static_cast<unsigned>(all) / static_cast<unsigned>(grid)) : i * all / grid;
-    };
-    long long at = share(blockIdx.x);
-    const long long end = share(blockIdx.x + 1);
+    const bool brief = paged_brief(all);
+    long long at = paged_share(blockIdx.x, all, grid, brief);
+    const long long end = paged_share(blockIdx.x + 1, all, grid, brief);
     int b = 0;
     long long first = 0;  // the row's index of sequence b's first unit
     for (int b0 = 0; b0 < pc.batch; b0 += 32) {
@@ -667,11 +662,7 @@ __global__ void __launch_bounds__(128, (AttnShape<C, D, WIDE>::kCtas)) attn_deco
         if (whole) continue;
 
         // The pair's last CTA to come here merges all its partials, in CTA order.
-        auto owner = [&](long long unit) {
-            const long long v = (unit + 1) * grid - 1;
-            return brief ? static_cast<int>(static_cast<unsigned>(v) / static_cast<unsigned>(all)) : static_cast<int>(v / all);
-        };
-        const int cta0 = owner(pair_first), cta1 = owner(pair_first + nu - 1);
+        const int cta0 = paged_owner(pair_first, all, grid, brief), cta1 = paged_owner(pair_first + nu - 1, all, grid, brief);
         int* ticket = p.tickets + static_cast<int64_t>(seq) * pairs + pair;
         __syncthreads();  // the partial is written; one thread's fence carries it to the others' reads
         if (threadIdx.x == 0) {
@@ -748,7 +739,7 @@ cudaError_t attend_shape(AttnParams p, int num_sms, cudaStream_t s) {
     p.blocks = (p.group - 1) / S::kRows + 1;
     const long long longest = static_cast<long long>(p.pc.max_pages) * p.pc.page_size;
     const long long chunks = ((longest - 1) / kChunk + 1) * p.pc.batch * p.pc.kv_heads * p.blocks;
-    const long long most = std::min(num_sms * S::kCtas, kAttnMaxCtas);
+    const long long most = std::min(num_sms * S::kCtas, kPagedMaxCtas);
     count_launch();
     attn_decode_paged_kernel<C, D, WIDE>
         <<<static_cast<int>(std::min(chunks, most)), 128, S::kSmemFloats * sizeof(float), s>>>(p);
