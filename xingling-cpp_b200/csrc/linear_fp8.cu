@@ -223,33 +223,65 @@ __device__ __forceinline__ void store_rows(const unsigned long long (&acc)[64], 
             }
         }
         __syncwarp();
+        // what y holds is read for all rows before the first is written: one memory round trip, not one a row
         if (vec && o0 + 16 <= wide) {
-            constexpr int kLanes = 16 / kPer;  // lanes a row
+            constexpr int kLanes = 16 / kPer, kTurns = kLanes;  // lanes a row; rows 32 / kLanes at a time
+            T* dst = y + static_cast<size_t>(tok0 + lane / kLanes) * wide + o0 + lane % kLanes * kPer;
+            const size_t turn = static_cast<size_t>(32 / kLanes) * wide;
+            uint4 old[kTurns];
 #pragma unroll
-            for (int r0 = 0; r0 < 32; r0 += 32 / kLanes) {
-                const int r = r0 + lane / kLanes, c = lane % kLanes * kPer;
+            for (int i = 0; i < kTurns; ++i) {
+                old[i] = make_uint4(0u, 0u, 0u, 0u);
+                if (p.mode == kGemvResidual && i * (32 / kLanes) + lane / kLanes < rows)
+                    old[i] = *reinterpret_cast<const uint4*>(dst + i * turn);
+            }
+#pragma unroll
+            for (int i = 0; i < kTurns; ++i) {
+                const int r = i * (32 / kLanes) + lane / kLanes;
                 if (r < rows) {
-                    const float* src = st + r * kStagePitch + c;
-                    T* dst = y + static_cast<size_t>(tok0 + r) * wide + o0 + c;
-                    uint4 out;
-                    T* e = reinterpret_cast<T*>(&out);
-                    if (p.mode == kGemvResidual) {
-                        out = *reinterpret_cast<const uint4*>(dst);
+                    const float* src = st + r * kStagePitch + lane % kLanes * kPer;
+                    T* e = reinterpret_cast<T*>(&old[i]);
 #pragma unroll
-                        for (int i = 0; i < kPer; ++i) e[i] = from_float<T>(to_float(e[i]) + src[i]);
-                    } else {
-#pragma unroll
-                        for (int i = 0; i < kPer; ++i) e[i] = from_float<T>(src[i]);
-                    }
-                    *reinterpret_cast<uint4*>(dst) = out;
+                    for (int k = 0; k < kPer; ++k)
+                        e[k] = from_float<T>(p.mode == kGemvResidual ? to_float(e[k]) + src[k] : src[k]);
+                    *reinterpret_cast<uint4*>(dst + i * turn) = old[i];
                 }
             }
         } else {
+            // 16 lanes a row, or rows of whole words: 8 lanes with 2 outputs (16-bit y)
+            const bool two = sizeof(T) == 2 && wide % 2 == 0;
+            const int per = two ? 2 : 1, lanes = 16 / per, apart = 32 / lanes;
+            const int r0 = lane / lanes, c = lane % lanes * per;
+            T* dst = y + static_cast<size_t>(tok0 + r0) * wide + o0 + c;
+            const float* src = st + r0 * kStagePitch + c;
+            const size_t turn = static_cast<size_t>(apart) * wide;
+            const int mine = o0 + c < wide ? (rows - r0 + apart - 1) / apart : 0;
+            if (p.mode == kGemvResidual) {
+#pragma unroll 1
+                for (int t0 = 0; t0 < mine; t0 += 8) {
+                    float old[8];
+#pragma unroll
+                    for (int half = 0; half < 2; ++half) {
+                        if (half >= per) break;
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) old[i] = t0 + i < mine ? to_float(dst[(t0 + i) * turn + half]) : 0.0f;
+#pragma unroll
+                        for (int i = 0; i < 8; ++i)
+                            if (t0 + i < mine)
+                                dst[(t0 + i) * turn + half] = from_float<T>(old[i] + src[(t0 + i) * apart * kStagePitch + half]);
+                    }
+                }
+            } else if (two) {
+                if constexpr (sizeof(T) == 2) {
 #pragma unroll 4
-            for (int r0 = 0; r0 < rows; r0 += 2) {
-                const int r = r0 + lane / 16, c = lane % 16;
-                if (r < rows && o0 + c < wide)
-                    put(y + static_cast<size_t>(tok0 + r) * wide + o0 + c, st[r * kStagePitch + c], p.mode);
+                    for (int i = 0; i < mine; ++i) {
+                        const float* v = src + i * apart * kStagePitch;
+                        *reinterpret_cast<uint32_t*>(dst + i * turn) = pack_pair(v[0], v[1], T{});
+                    }
+                }
+            } else {
+#pragma unroll 4
+                for (int i = 0; i < mine; ++i) dst[i * turn] = from_float<T>(src[i * apart * kStagePitch]);
             }
         }
         __syncwarp();
@@ -698,16 +730,27 @@ __global__ void __launch_bounds__(Few<N>::kThreads, Few<N>::kCtas)
                 T* y = static_cast<T*>(p.y);
                 const bool swiglu = p.mode == kGemvSwiGLU;
 #pragma unroll
-                for (int i = 0; i < N; ++i) {
-                    const size_t row = static_cast<size_t>(tok0 + i);
-                    const float2 v2 = unpack2(acc[i / 2]);
-                    const float v = (i & 1 ? v2.y : v2.x) + bias;
-                    if (i >= rows) {
-                    } else if (swiglu) {
-                        const float c = __shfl_xor_sync(0xffffffffu, v, 1);
-                        if (!(lane & 1) && j < p.m) y[row * (p.m >> 1) + (j >> 1)] = from_float<T>(silu_fast(v) * c);
-                    } else if (j < p.m) {
-                        put(y + row * p.m + j, v, p.mode);
+                for (int i0 = 0; i0 < N; i0 += 16) {
+                    // what y holds is read for 16 tokens before the first is written
+                    float old[16];
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) {
+                        old[i] = 0.0f;
+                        if (p.mode == kGemvResidual && i0 + i < rows && j < p.m)
+                            old[i] = to_float(y[static_cast<size_t>(tok0 + i0 + i) * p.m + j]);
+                    }
+#pragma unroll
+                    for (int i = i0; i < i0 + 16; ++i) {
+                        const size_t row = static_cast<size_t>(tok0 + i);
+                        const float2 v2 = unpack2(acc[i / 2]);
+                        const float v = (i & 1 ? v2.y : v2.x) + bias;
+                        if (i >= rows) {
+                        } else if (swiglu) {
+                            const float c = __shfl_xor_sync(0xffffffffu, v, 1);
+                            if (!(lane & 1) && j < p.m) y[row * (p.m >> 1) + (j >> 1)] = from_float<T>(silu_fast(v) * c);
+                        } else if (j < p.m) {
+                            y[row * p.m + j] = from_float<T>(old[i - i0] + v);
+                        }
                     }
                 }
             } else {
@@ -758,7 +801,10 @@ __global__ void __launch_bounds__(Few<N>::kThreads, Few<N>::kCtas)
                 T* dst = y + static_cast<size_t>(tok) * p.m + j;
 #pragma unroll
                 for (int i = 0; i < 4; ++i)
-                    if (j + i < p.m) put(dst + i, o[i], p.mode);
+                    if (p.mode == kGemvResidual && j + i < p.m) o[i] += to_float(dst[i]);
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    if (j + i < p.m) dst[i] = from_float<T>(o[i]);
             }
         }
     }
