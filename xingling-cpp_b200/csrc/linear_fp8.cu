@@ -190,10 +190,10 @@ __device__ __forceinline__ void put(T* dst, float v, int mode) {
 // 32 tokens x 128 features in registers (a token a lane) to y, 16 outputs a
 // row at a time through the warp's staging rows, so that stores are 16 bytes
 // a lane along the rows.  bias: the warp's 128 values in shared memory.
-template <typename T>
+template <typename T, int MODE>
 __device__ __forceinline__ void store_rows(const unsigned long long (&acc)[64], const LinearParams& p, int tok0, int j0,
                                            float* st, const float4* bias, int lane) {
-    const bool swiglu = p.mode == kGemvSwiGLU;
+    constexpr bool swiglu = MODE == kGemvSwiGLU;
     const int wide = swiglu ? p.m / 2 : p.m;
     const bool vec = (static_cast<size_t>(wide) * sizeof(T)) % 16 == 0;
     const int rows = min(32, p.n - tok0);
@@ -232,23 +232,36 @@ __device__ __forceinline__ void store_rows(const unsigned long long (&acc)[64], 
             constexpr int kLanes = 16 / kPer, kTurns = kLanes;  // lanes a row; rows 32 / kLanes at a time
             T* dst = y + static_cast<size_t>(tok0 + lane / kLanes) * wide + o0 + lane % kLanes * kPer;
             const size_t turn = static_cast<size_t>(32 / kLanes) * wide;
-            uint4 old[kTurns];
+            if constexpr (MODE == kGemvResidual) {
+                uint4 old[kTurns];
 #pragma unroll
-            for (int i = 0; i < kTurns; ++i) {
-                old[i] = make_uint4(0u, 0u, 0u, 0u);
-                if (p.mode == kGemvResidual && i * (32 / kLanes) + lane / kLanes < rows)
-                    old[i] = *reinterpret_cast<const uint4*>(dst + i * turn);
-            }
+                for (int i = 0; i < kTurns; ++i) {
+                    old[i] = make_uint4(0u, 0u, 0u, 0u);
+                    if (i * (32 / kLanes) + lane / kLanes < rows) old[i] = *reinterpret_cast<const uint4*>(dst + i * turn);
+                }
 #pragma unroll
-            for (int i = 0; i < kTurns; ++i) {
-                const int r = i * (32 / kLanes) + lane / kLanes;
-                if (r < rows) {
-                    const float* src = st + r * kStagePitch + lane % kLanes * kPer;
-                    T* e = reinterpret_cast<T*>(&old[i]);
+                for (int i = 0; i < kTurns; ++i) {
+                    const int r = i * (32 / kLanes) + lane / kLanes;
+                    if (r < rows) {
+                        const float* src = st + r * kStagePitch + lane % kLanes * kPer;
+                        T* e = reinterpret_cast<T*>(&old[i]);
 #pragma unroll
-                    for (int k = 0; k < kPer; ++k)
-                        e[k] = from_float<T>(p.mode == kGemvResidual ? to_float(e[k]) + src[k] : src[k]);
-                    *reinterpret_cast<uint4*>(dst + i * turn) = old[i];
+                        for (int k = 0; k < kPer; ++k) e[k] = from_float<T>(to_float(e[k]) + src[k]);
+                        *reinterpret_cast<uint4*>(dst + i * turn) = old[i];
+                    }
+                }
+            } else {
+#pragma unroll
+                for (int i = 0; i < kTurns; ++i) {
+                    const int r = i * (32 / kLanes) + lane / kLanes;
+                    if (r < rows) {
+                        const float* src = st + r * kStagePitch + lane % kLanes * kPer;
+                        uint4 out;
+                        T* e = reinterpret_cast<T*>(&out);
+#pragma unroll
+                        for (int k = 0; k < kPer; ++k) e[k] = from_float<T>(src[k]);
+                        *reinterpret_cast<uint4*>(dst + i * turn) = out;
+                    }
                 }
             }
         } else {
@@ -260,7 +273,7 @@ __device__ __forceinline__ void store_rows(const unsigned long long (&acc)[64], 
             const float* src = st + r0 * kStagePitch + c;
             const size_t turn = static_cast<size_t>(apart) * wide;
             const int mine = o0 + c < wide ? (rows - r0 + apart - 1) / apart : 0;
-            if (p.mode == kGemvResidual) {
+            if (MODE == kGemvResidual) {
 #pragma unroll 1
                 for (int t0 = 0; t0 < mine; t0 += 8) {
                     float old[8];
@@ -292,7 +305,9 @@ __device__ __forceinline__ void store_rows(const unsigned long long (&acc)[64], 
     }
 }
 
-template <typename T>
+// MODE at compile time: a tile's store runs once or a few times a call, and the code of the other modes beside it cost
+// instruction fetch.
+template <typename T, int MODE>
 __global__ void __launch_bounds__(Pair::kThreads, 1)
     linear_fp8_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_w,
                            const LinearParams p) {
@@ -468,7 +483,7 @@ __global__ void __launch_bounds__(Pair::kThreads, 1)
 #pragma unroll
                 for (int i = 0; i < 4; ++i) sb[32 * i + lane] = bias[i];
                 __syncwarp();
-                store_rows<T>(acc, p, tok0, j0, st, reinterpret_cast<const float4*>(sb), lane);
+                store_rows<T, MODE>(acc, p, tok0, j0, st, reinterpret_cast<const float4*>(sb), lane);
             }
         }
         asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
@@ -512,17 +527,17 @@ cudaError_t launch_linear(LinearKernel kernel, std::atomic<unsigned long long>& 
     return cudaLaunchKernelEx(&cfg, kernel, mx, mw, p);
 }
 
-template <typename T>
+template <typename T, int MODE>
 cudaError_t launch_pairs(const CUtensorMap& mx, const CUtensorMap& mw, const LinearParams& p, int grid, cudaStream_t s) {
     // the warpgroups' register shares have to fit what the CTA launches with, or the larger one never comes
     static const bool fits = [] {
         cudaFuncAttributes a{};
-        return cudaFuncGetAttributes(&a, linear_fp8_pair_kernel<T>) == cudaSuccess &&
+        return cudaFuncGetAttributes(&a, linear_fp8_pair_kernel<T, MODE>) == cudaSuccess &&
                a.numRegs * Pair::kThreads >= 128 * 40 + 256 * 232;
     }();
     if (!fits) return cudaErrorInvalidConfiguration;
     static std::atomic<unsigned long long> allowed{0};
-    return launch_linear(linear_fp8_pair_kernel<T>, allowed, mx, mw, p, grid, Pair::kThreads, 2,
+    return launch_linear(linear_fp8_pair_kernel<T, MODE>, allowed, mx, mw, p, grid, Pair::kThreads, 2,
                          p.stages * Pair::kStage + Pair::kStoreBytes + kBarBytes + 1024, s);
 }
 
@@ -1045,7 +1060,10 @@ cudaError_t launch_tokens(LinearParams& p, const uint8_t* xq, size_t ldx, const 
     cudaError_t e = make_byte_map(&mx, xq, n, k, ldx, 128);
     if (e == cudaSuccess) e = make_byte_map(&mw, wq, m, k, ldw, 128);
     if (e != cudaSuccess) return e;
-    return launch_pairs<T>(mx, mw, p, 2 * static_cast<int>(std::min<long long>(t2, num_sms / 2)), s);
+    const int grid = 2 * static_cast<int>(std::min<long long>(t2, num_sms / 2));
+    if (p.mode == kGemvSwiGLU) return launch_pairs<T, kGemvSwiGLU>(mx, mw, p, grid, s);
+    if (p.mode == kGemvResidual) return launch_pairs<T, kGemvResidual>(mx, mw, p, grid, s);
+    return launch_pairs<T, kGemvPlain>(mx, mw, p, grid, s);
 }
 
 }  // namespace
