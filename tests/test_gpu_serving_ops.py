@@ -303,6 +303,23 @@ def test_linear_infinite_and_nan_scales_stay_in_their_rows(torch):
     assert bad[133].all() and not bad[:133].any() and not bad[134:].any()
 
 
+@pytest.mark.parametrize("n,m,k", [(3, 520, 384), (20, 520, 384), (100, 520, 384), (1100, 2600, 256)])
+def test_linear_nan_operands(torch, n, m, k):
+    """An e4m3 NaN makes its token's row, or its weight row's column, NaN, and nothing else."""
+    g = gen(torch, n)
+    (dx, x), (dw, w) = random_fp8(torch, n, k, g), random_fp8(torch, m, k, g)
+    dx[n - 1, 130], dw[m - 3, 7] = 0x7F, 0xFF
+    xs, ws = torch.full((n, k // 128), 0.01, device="cuda"), torch.full(((m + 127) // 128, k // 128), 0.01, device="cuda")
+    y = torch.empty((n, m), device="cuda")
+    X.check(X.lib().xl_op_linear_fp8(0, 0, X.ptr(dx), dx.stride(0), X.ptr(xs), X.ptr(dw), dw.stride(0), X.ptr(ws), None,
+                                     X.ptr(y), n, m, k, X.stream()))
+    torch.cuda.synchronize()
+    want = torch.zeros((n, m), dtype=torch.bool)
+    want[n - 1] = True
+    want[:, m - 3] = True
+    assert torch.equal(y.isnan().cpu(), want)
+
+
 # ---- the paged cache ------------------------------------------------------------------------------------------------
 
 class Paged:
@@ -411,6 +428,9 @@ ATTEND = [
     (0, 0, 1, 1, 64, 256, [2047]),
     (1, 1, 8, 1, 128, 16, [3000]),
     (2, 2, 2, 1, 128, 48, [-1, -1]),
+    (0, 0, 12, 1, 128, 8, [0, 300, 64]),
+    (0, 0, 26, 2, 64, 16, [90, 1]),
+    (1, 2, 10, 1, 128, 32, [65, 400]),
 ]
 
 
