@@ -1,0 +1,114 @@
+"""The 8-bit projections and the paged cache where ordinary values do not reach:
+scores far apart, infinities and NaN in the cache, batches whose work crosses
+sequences, ties, and the ends of the floats' range.  The bounds are those of
+test_gpu_serving_ops.py, whose helpers are used."""
+import math
+
+import pytest
+
+import test_gpu_serving_ops as T
+import xl_capi as X
+
+pytestmark = pytest.mark.gpu
+
+U = T.U
+CACHES = pytest.mark.parametrize("cache", [0, 1, 2], ids=["fp32", "bf16", "fp16"])
+
+
+@pytest.fixture(scope="module")
+def torch(built):
+    import torch
+
+    torch.cuda.init()
+    return torch
+
+
+# ---- attention -----------------------------------------------------------------------------------------------------
+
+class Pool:
+    """A shuffled pool for many sequences, filled on the device; positions past each sequence's rows hold NaN."""
+
+    def __init__(self, torch, dtype, lens, kv, d, page, seed):
+        self.page, self.kv, self.d = page, kv, d
+        g = torch.Generator(device="cuda").manual_seed(seed)
+        need = torch.tensor([(n + page - 1) // page for n in lens])
+        total, wide = int(need.sum()) + 2, max(1, int(need.max()))
+        order = torch.randperm(total, generator=torch.Generator().manual_seed(seed))
+        column = torch.arange(wide)
+        index = (need.cumsum(0) - need)[:, None] + column
+        self.table = torch.where(column < need[:, None], order[index.clamp(max=total - 1)], 1 << 30).int()
+        self.dt = self.table.cuda()
+        t = T.types(torch)[dtype]
+        self.k, self.v = (torch.empty((total, kv, page, d), dtype=t, device="cuda").normal_(generator=g) for _ in range(2))
+        for b, n in enumerate(lens):
+            if n % page:
+                last = int(self.table[b, n // page])
+                self.k[last, :, n % page:] = math.nan
+                self.v[last, :, n % page:] = math.inf
+        self.c = X.PagedKV(self.k.data_ptr(), self.v.data_ptr(), self.dt.data_ptr(), dtype, len(lens), kv, d, page, wide, total)
+
+    def rows(self, b, n):
+        """Positions 0 .. n - 1 of sequence b as views: [kv][n][d] copies in 64 bits."""
+        pages = self.dt[b, :(n + self.page - 1) // self.page].long()
+        return tuple(x[pages].permute(1, 0, 2, 3).reshape(self.kv, -1, self.d)[:, :n].double() for x in (self.k, self.v))
+
+    def put(self, which, b, pos, value):
+        """value (a row of d, or what broadcasts to it) at position pos of sequence b, in all heads."""
+        (self.k if which == "k" else self.v)[int(self.table[b, pos // self.page]), :, pos % self.page] = value
+
+
+def check(torch, pool, qkv, rope, b, n, out, heads):
+    """Sequence b's output against 64 bits over what the cache holds, the kinds of its values (finite, an infinity, NaN)
+    among them."""
+    d, kv, group = pool.d, pool.kv, heads // pool.kv
+    row = qkv[b].double().view(heads + 2 * kv, d)
+    q = row[:heads]
+    keys, values = pool.rows(b, n + 1)
+    big = q.abs() + q.abs().roll(d // 2, -1) if rope is not None else q.abs()
+    if rope is not None:
+        q = T.rotate(torch, q, rope[n])
+    q, big = q.view(kv, group, d), big.view(kv, group, d)
+    s = torch.einsum("kgd,knd->kgn", q, keys) / math.sqrt(d)
+    w = torch.softmax(s, -1)
+    want = torch.empty((kv, group, d), dtype=torch.float64, device="cuda")
+    reach = torch.empty_like(want)
+    finite = torch.where(values.isfinite(), values, 0.0).abs()
+    for h in range(kv):  # products and a sum, so that 0 x inf shows as it does in the definition
+        for i in range(group):
+            want[h, i] = (w[h, i][:, None] * values[h]).sum(0)
+            reach[h, i] = (w[h, i][:, None] * finite[h]).sum(0)
+    size = torch.where(keys.isfinite(), keys, 0.0).abs()
+    ds = ((d + 8) * 2 * U + 8 * U + 2.0 ** -21) * torch.einsum("kgd,knd->kgn", big, size).amax(-1, keepdim=True) / math.sqrt(d)
+    tol = (2 * ds + 2.0 ** -16 + (n + 17) * 2 * U + 2.0 ** -20) * reach
+    got = out[b].double().view(kv, group, d)
+    assert torch.equal(got.isnan(), want.isnan()), (b, int(got.isnan().sum()), int(want.isnan().sum()))
+    inf = want.isinf()
+    assert torch.equal(got.isinf(), inf) and torch.equal(got[inf], want[inf]), b
+    ok = want.isfinite()
+    off = (got - want).abs() - tol - T.half_step(torch, out.dtype) * (want.abs() + tol) - torch.finfo(out.dtype).tiny
+    assert (off[ok] <= 0).all(), (b, float(off[ok].max()), float(tol[ok].max()))
+
+
+@CACHES
+@pytest.mark.parametrize("heads,kv,d", [(4, 2, 64), (10, 1, 128)])
+@pytest.mark.parametrize("gap", [12, 16, 18, 21, 25])
+def test_attend_small_weights(torch, cache, heads, kv, d, gap):
+    """One position stands `gap` above the others and holds a value of zero, so the small weights are all of the output."""
+    n = 1500
+    p = Pool(torch, cache, [n + 1] * 3, kv, d, 16, seed=gap)
+    for b, spot in enumerate((0, 700, n)):
+        p.k[p.table[b].long().cuda(), :, :, 0] = 0.0
+        p.put("k", b, spot, torch.eye(1, d, device="cuda")[0] * gap)
+        p.put("v", b, spot, 0.0)
+    qkv = torch.randn((3, (heads + 2 * kv) * d), generator=T.gen(torch, 2))
+    rows = qkv.view(3, heads + 2 * kv, d)
+    rows[:, :heads] *= 0.01
+    rows[:, :heads, 0] = math.sqrt(d)
+    rows[:, heads:, 0] = 0.0
+    rows[2, heads:heads + kv] = torch.eye(1, d)[0] * gap
+    rows[2, heads + kv:] = 0.0
+    dq, out = qkv.cuda(), torch.empty((3, heads * d), device="cuda")
+    pos = torch.full((3,), n, dtype=torch.int32, device="cuda")
+    T.attend(torch, p, 0, dq, None, pos, out, heads, T.workspace(torch, p.c, heads))
+    for b in range(3):
+        check(torch, p, dq, None, b, n, out, heads)

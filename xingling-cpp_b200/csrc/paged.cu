@@ -94,10 +94,13 @@ __global__ void __launch_bounds__(kAppendThreads) kv_append_paged_kernel(const P
 // shared memory in that layout; the weights change from one MMA's result to
 // the next one's operand by an 8 x 8 transpose in registers (movmatrix).
 //
-// Precision: queries are split in two 16-bit halves (for fp16 scaled by a power
-// of two first), and so are the weights, which leaves 2^-17 of error
-// where rounding them would leave 2^-9; an fp32 cache runs as three TF32
-// products of split operands.  Sums, maxima and the running output are fp32.
+// Precision: queries are split in two 16-bit halves, and so are the weights,
+// which leaves 2^-17 (bf16) or 2^-23 (fp16) of error where rounding them would
+// leave 2^-9 or 2^-12; an fp32 cache runs as three TF32 products of split
+// operands.  fp16 has no value below 2^-24 and none above 65504: what is split
+// for it is scaled by powers of two, the low half by one more, so that a weight
+// keeps its 2^-23 down to 2^-29 of the largest (e^-20) and an absolute 2^-52
+// below.  Sums, maxima and the running output are fp32.
 //
 // 64 sequences up to 8192 (32 heads on 8 of 128, bf16): 202 us, 5.4 TB/s; one
 // of 131072: 101 us, 5.3 TB/s.  8 sequences up to 768 (24 heads of 64, fp32):
@@ -183,12 +186,19 @@ __device__ __forceinline__ int row_exponent(uint32_t bits) {
     return bits == 0u || bits >= 0x7f800000u ? 0 : max(-120, min(120, e));
 }
 
-// Two values as a pair of 16-bit halves: v = hi + lo up to 2^-17 (bf16) or 2^-22 (fp16) of it.
+// What the low half is scaled by: the rounding of the high one is 2^-12 of it at most.
+template <typename C>
+constexpr float kLowUp = kScaled<C> ? 4096.0f : 1.0f;
+// What the weights (at most 1) are scaled by: up to 2^15 is below fp16's largest value.
+template <typename C>
+constexpr float kWeightUp = kScaled<C> ? 32768.0f : 1.0f;
+
+// Two values as a pair of 16-bit halves: v = hi + lo / kLowUp up to 2^-17 (bf16) or 2^-23 (fp16, from 2^-14 on) of it.
 template <typename C>
 __device__ __forceinline__ void split16(float a, float b, uint32_t& hi, uint32_t& lo) {
     const float ha = to_float(from_float<C>(a)), hb = to_float(from_float<C>(b));
     hi = pack_pair(ha, hb, C{});
-    lo = pack_pair(a - ha, b - hb, C{});
+    lo = pack_pair((a - ha) * kLowUp<C>, (b - hb) * kLowUp<C>, C{});
 }
 // v = hi + lo for TF32 products: hi to nearest, so that what lo loses (it is
 // cut to 11 bits) has no sign of its own.
@@ -532,7 +542,8 @@ __global__ void __launch_bounds__(128, (AttnShape<C, D, WIDE>::kCtas)) attn_deco
 #pragma unroll
             for (int h = 0; h < S::kHalves; ++h) {
 #pragma unroll
-                for (int j = 0; j < 4; ++j) s[h][j] = (s[h][j] + also[h][j] + more[h][j]) * back[h][j & 1];
+                for (int j = 0; j < 4; ++j)
+                    s[h][j] = (s[h][j] + also[h][j] + more[h][j] * (1.0f / kLowUp<C>)) * back[h][j & 1];
                 if (x0 + kTile > pos + 1) {
 #pragma unroll
                     for (int j = 0; j < 4; ++j)
@@ -575,18 +586,18 @@ __global__ void __launch_bounds__(128, (AttnShape<C, D, WIDE>::kCtas)) attn_deco
                         wl[h][2 * n] = tf32_lo(w0, wh[h][2 * n]), wl[h][2 * n + 1] = tf32_lo(w1, wh[h][2 * n + 1]);
                     } else {
                         uint32_t hi, lo;
-                        split16<C>(s[h][2 * n], s[h][2 * n + 1], hi, lo);
+                        split16<C>(s[h][2 * n] * kWeightUp<C>, s[h][2 * n + 1] * kWeightUp<C>, hi, lo);
                         wh[h][n] = transpose8(hi), wl[h][n] = transpose8(lo);
                     }
                 }
 #pragma unroll
             for (int i = 0; i < D / 16; ++i) {
                 const int ch = i / (S::kVec / 2), e = i % (S::kVec / 2);
-                float o[S::kHalves][4];
+                float o[S::kHalves][4], low[S::kHalves][4];  // low: of the low halves, where they are scaled
 #pragma unroll
                 for (int h = 0; h < S::kHalves; ++h)
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) o[h][j] = 0.0f;
+                    for (int j = 0; j < 4; ++j) o[h][j] = low[h][j] = 0.0f;
                 if constexpr (S::k32) {
                     // position 2t is the MMA's k = t, 2t + 1 its k = t + 4; columns 2e and 2e + 1 its rows g and g + 8
 #pragma unroll
@@ -609,14 +620,14 @@ __global__ void __launch_bounds__(128, (AttnShape<C, D, WIDE>::kCtas)) attn_deco
                                            __byte_perm(z, u, 0x7632)};
 #pragma unroll
                     for (int h = 0; h < S::kHalves; ++h) {
-                        mma16(o[h], a, wl[h][0], wl[h][1], C{});
+                        mma16(kScaled<C> ? low[h] : o[h], a, wl[h][0], wl[h][1], C{});
                         mma16(o[h], a, wh[h][0], wh[h][1], C{});
                     }
                 }
 #pragma unroll
                 for (int h = 0; h < S::kHalves; ++h)
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) acc[h][i][j] += o[h][j];
+                    for (int j = 0; j < 4; ++j) acc[h][i][j] += kScaled<C> ? o[h][j] + low[h][j] * (1.0f / kLowUp<C>) : o[h][j];
             }
             load_v(next);
         }
@@ -636,8 +647,8 @@ __global__ void __launch_bounds__(128, (AttnShape<C, D, WIDE>::kCtas)) attn_deco
 #pragma unroll
                 for (int i = 0; i < D / 16; ++i) {
                     const int d = (i / (S::kVec / 2)) * 8 * S::kVec + S::kVec * g + 2 * (i % (S::kVec / 2));
-                    row[d] = acc[h][i][j];
-                    row[d + 1] = acc[h][i][j + 2];
+                    row[d] = acc[h][i][j] * (1.0f / kWeightUp<C>);
+                    row[d + 1] = acc[h][i][j + 2] * (1.0f / kWeightUp<C>);
                 }
                 if (g == 0) row[D] = top[h][j], row[D + 1] = l;
             }
