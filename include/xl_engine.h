@@ -437,8 +437,9 @@ XL_API int xl_op_kv_append_paged(const xl_paged_kv* cache, int dtype, const void
  * as the cache holds them (scale head_dim^-1/2).  heads is a multiple of
  * kv_heads; query head h reads key/value head h / (heads / kv_heads).
  * Statistics and sums are fp32; queries and weights meet a bf16 cache with 16
- * bits (2^-17 relative), an fp16 one with 22 (weights below 2^-29 of the largest
- * with 2^-52 of it), an fp32 one with 21 to 22.
+ * bits (2^-17 relative), an fp16 one with 22 (what is below 2^-28 of the largest
+ * weight, or of the query's largest element, with 2^-51 of that), an fp32 one
+ * with 21 to 22.
  * pos[b] = -1: no sequence, zeros.  Any other position out of range, or a page
  * id outside [0, num_pages) among the pages needed: NaN outputs for that
  * sequence, and nothing is read or written through that position or page.

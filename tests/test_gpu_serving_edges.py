@@ -112,3 +112,20 @@ def test_attend_small_weights(torch, cache, heads, kv, d, gap):
     T.attend(torch, p, 0, dq, None, pos, out, heads, T.workspace(torch, p.c, heads))
     for b in range(3):
         check(torch, p, dq, None, b, n, out, heads)
+
+
+def test_attend_queries_of_uneven_size(torch):
+    """Query elements far below the row's largest count in full where the keys are small at the large ones."""
+    heads, kv, d, n = 4, 2, 64, 400
+    p = Pool(torch, 2, [n + 1], kv, d, 16, seed=4)
+    p.k[..., 0] = 0.0
+    p.k[..., 1:] *= 100
+    qkv = torch.randn((1, (heads + 2 * kv) * d), generator=T.gen(torch, 3))
+    rows = qkv.view(1, heads + 2 * kv, d)
+    rows[:, :heads] *= 2e-3
+    rows[:, :heads, 0] = 3e4
+    rows[:, heads:heads + kv, 0] = 0.0
+    dq, out = qkv.cuda(), torch.empty((1, heads * d), device="cuda")
+    pos = torch.tensor([n], dtype=torch.int32, device="cuda")
+    T.attend(torch, p, 0, dq, None, pos, out, heads, T.workspace(torch, p.c, heads))
+    check(torch, p, dq, None, 0, n, out, heads)

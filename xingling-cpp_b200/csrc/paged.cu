@@ -176,14 +176,15 @@ __device__ __forceinline__ uint4 load_shared(const uint4* p) {
     return v;
 }
 
-// fp16 holds 5 exponent bits: a query row is scaled by a power of two so that its largest value is in [1, 2).
+// fp16 holds 5 exponent bits: a query row is scaled by 2^-row_exponent so that its largest value is in [2^14, 2^15), which
+// leaves an element 2^-28 of that its 2^-23.  (A row below 2^-112 is scaled by less; its scores are zeros beside 1.)
 template <typename C>
 constexpr bool kScaled = false;
 template <>
 constexpr bool kScaled<__half> = true;
 __device__ __forceinline__ int row_exponent(uint32_t bits) {
-    const int e = static_cast<int>(bits >> 23) - 127;
-    return bits == 0u || bits >= 0x7f800000u ? 0 : max(-120, min(120, e));
+    const int e = static_cast<int>(bits >> 23) - 127 - 14;
+    return bits == 0u || bits >= 0x7f800000u ? 0 : max(-126, e);
 }
 
 // What the low half is scaled by: the rounding of the high one is 2^-12 of it at most.
