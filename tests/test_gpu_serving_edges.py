@@ -129,3 +129,105 @@ def test_attend_queries_of_uneven_size(torch):
     pos = torch.tensor([n], dtype=torch.int32, device="cuda")
     T.attend(torch, p, 0, dq, None, pos, out, heads, T.workspace(torch, p.c, heads))
     check(torch, p, dq, None, 0, n, out, heads)
+
+
+def special(torch, p, rows, b, n, what, heads):
+    """Makes sequence b (last position n) hold `what`; element 0 of every query is -1, element 1 is 4 sqrt(d)."""
+    kv, d, mid = p.kv, p.d, n // 2
+    unit = torch.zeros(d, device="cuda")
+    if what == "key_out":  # a score of minus infinity: weight 0
+        unit[0] = math.inf
+        p.put("k", b, mid, unit)
+    elif what == "keys_out":  # the first chunk of 64 positions and part of the second
+        unit[0] = math.inf
+        for t in range(min(80, n)):
+            p.put("k", b, t, unit)
+    elif what == "all_out":  # nothing is left: 0 / 0
+        unit[0] = math.inf
+        for t in range(n):
+            p.put("k", b, t, unit)
+        rows[b, heads:heads + kv, 0] = math.inf
+    elif what == "key_in":  # a score of infinity: inf - inf in the softmax
+        unit[0] = -math.inf
+        p.put("k", b, mid, unit)
+    elif what == "key_nan":
+        unit[3] = math.nan
+        p.put("k", b, mid, unit)
+    elif what == "value":
+        unit[3], unit[5], unit[7] = math.inf, -math.inf, math.inf
+        p.put("v", b, mid, unit)
+        unit[3], unit[5], unit[7] = 0.0, 0.0, -math.inf
+        p.put("v", b, 0, unit)
+    elif what == "value_far":  # at a weight of e^-60, e^-95 and, in the last position, e^-130
+        for t, (down, column) in {0: (60, 2), mid: (95, 3), n: (130, 4)}.items():
+            key = unit.clone()
+            key[1], value = -down / 4.0, unit.clone()
+            value[column] = math.inf
+            if t == n:
+                rows[b, heads:heads + kv] = key.cpu()
+                rows[b, heads + kv:] = value.cpu()
+            else:
+                p.put("k", b, t, key)
+                p.put("v", b, t, value)
+    elif what == "value_out":  # 0 x inf
+        unit[0] = math.inf
+        p.put("k", b, mid, unit)
+        unit[0], unit[9] = 0.0, math.inf
+        p.put("v", b, mid, unit)
+    elif what == "value_nan":
+        unit[6] = math.nan
+        p.put("v", b, n - 1 if n else 0, unit)
+    elif what == "overflow":  # finite rows that a 16-bit cache stores as infinity
+        rows[b, heads + kv:, 8] = 1e5
+    else:
+        assert what == "plain"
+
+
+SPECIALS = ["plain", "key_out", "keys_out", "all_out", "key_in", "key_nan", "value", "value_far", "value_out", "value_nan",
+            "overflow"]
+
+
+@CACHES
+@pytest.mark.parametrize("heads,kv,d", [(4, 2, 64), (8, 1, 128), (12, 1, 64), (32, 2, 128)])
+@pytest.mark.parametrize("n,copies", [(1, 1), (90, 1), (700, 1), (90, 60)])
+def test_attend_infinities_and_nan(torch, cache, heads, kv, d, n, copies):
+    """Infinities and NaN in the cache, in sequences that one CTA takes, that several share, and (many of them) that
+    follow one another in one CTA."""
+    whats = SPECIALS * copies
+    p = Pool(torch, cache, [n + 1] * len(whats), kv, d, 16, seed=n)
+    p.k[..., 1] = 0.0
+    qkv = torch.randn((len(whats), (heads + 2 * kv) * d), generator=T.gen(torch, n))
+    rows = qkv.view(len(whats), heads + 2 * kv, d)
+    rows[:, :heads, 0], rows[:, :heads, 1], rows[:, heads:heads + kv, 1] = -1.0, 4 * math.sqrt(d), 0.0
+    for b, what in enumerate(whats):
+        special(torch, p, rows, b, n, what, heads)
+    dq = qkv.cuda()
+    pos = torch.full((len(whats),), n, dtype=torch.int32, device="cuda")
+    ws, outs = T.workspace(torch, p.c, heads), []
+    for _ in range(2):
+        out = torch.empty((len(whats), heads * d), device="cuda")
+        T.attend(torch, p, 0, dq, None, pos, out, heads, ws)
+        outs.append(out)
+    torch.cuda.synchronize()
+    for b in list(range(len(SPECIALS))) + list(range(len(whats) - len(SPECIALS), len(whats))) * (copies > 1):
+        check(torch, p, dq, None, b, n, out, heads)
+    assert torch.equal(outs[0].view(torch.int32), outs[1].view(torch.int32))
+
+
+def test_attend_infinite_query(torch):
+    """A query that is not finite makes its heads NaN and no other."""
+    heads, kv, d, n = 8, 2, 64, 130
+    for cache in (0, 1, 2):
+        p = Pool(torch, cache, [n + 1] * 2, kv, d, 16, seed=1)
+        qkv = torch.randn((2, (heads + 2 * kv) * d), generator=T.gen(torch, 6))
+        rows = qkv.view(2, heads + 2 * kv, d)
+        rows[0, 1, 5], rows[1, 6, 9] = math.inf, math.nan
+        dq, out = qkv.cuda(), torch.empty((2, heads * d), device="cuda")
+        pos = torch.full((2,), n, dtype=torch.int32, device="cuda")
+        T.attend(torch, p, 0, dq, None, pos, out, heads, T.workspace(torch, p.c, heads))
+        bad = out.view(2, heads, d).isnan()
+        want = torch.zeros_like(bad)
+        want[0, 1] = want[1, 6] = True
+        assert torch.equal(bad, want)
+        for b in range(2):
+            check(torch, p, dq, None, b, n, out, heads)

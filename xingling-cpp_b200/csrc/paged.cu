@@ -266,14 +266,107 @@ struct AttnShape {
     static constexpr int kCtas = D == 128 && (k32 || WIDE) ? 2 : 3;
 };
 
+// Where a CTA stands in its stretch and in a pair: kept in shared memory while the tiles run, which need the registers (64
+// sequences up to 8192, bf16: 204 us with all of it in registers, of which some were spilled, 187 us so).
+struct Stretch {
+    long long at, end, first, all, grid, pair_first;
+    int b, step, seq, pos, kh, h0, nh, c0, c1, nch, nu, pair;
+};
+
+// A warp's tiles of chunks c0 .. c1 again, in plain fp32, where their sums came out as an infinity or NaN.  Split operands
+// cannot tell what the definition says of those (0 x inf and inf - inf come up between the halves): here a score of minus
+// infinity is a weight of 0, an infinite value under a weight that is not 0 (however small) an infinite output, 0 x inf
+// and inf - inf NaN.  (All values infinite, 64 sequences up to 8192: 2.0 ms where finite ones take 0.19.)  2 heads and 4 positions at a time, D / 32 columns a lane; part: the warp's rows of D outputs,
+// maximum and sum, as the caller leaves them.
+template <typename C, int D>
+__device__ __forceinline__ void plain_part(const AttnParams& p, int seq, int kh, int h0, int nh, int pos, int c0, int c1,
+                                           bool bad, float* part) {
+    constexpr int kCols = D / 32, kHeads = 2, kRow = 4;  // columns lane + 32 i: i and i + kCols / 2 are a rotation's pair
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const PagedCache& pc = p.pc;
+    const int* table = pc.page_table + static_cast<int64_t>(seq) * pc.max_pages;
+    const C *kp = static_cast<const C*>(pc.k), *vp = static_cast<const C*>(pc.v);
+#pragma unroll 1
+    for (int r0 = 0; r0 < nh; r0 += kHeads) {  // past the last head: the last one again
+        float q[kHeads][kCols], o[kHeads][kCols], past[kHeads][kCols], top[kHeads], sum[kHeads];  // past: infinities, NaN
+#pragma unroll
+        for (int h = 0; h < kHeads; ++h) {
+            const int64_t src = seq * static_cast<int64_t>(p.heads + 2 * pc.kv_heads) * D +
+                                static_cast<int64_t>(h0 + min(r0 + h, nh - 1)) * D + lane;
+#pragma unroll
+            for (int i = 0; i < kCols; ++i) q[h][i] = load_io(p.qkv, src + 32 * i, p.io), o[h][i] = past[h][i] = 0.0f;
+            if (p.rope) {
+#pragma unroll
+                for (int i = 0; i < kCols / 2; ++i)
+                    rotate(q[h][i], q[h][i + kCols / 2], p.rope[static_cast<int64_t>(pos) * (D / 2) + lane + 32 * i]);
+            }
+            top[h] = -INFINITY, sum[h] = 0.0f;
+        }
+#pragma unroll 1
+        for (int c = c0; c < c1; ++c) {
+#pragma unroll 1
+            for (int t = 0; t < kTile; t += kRow) {
+                const int x0 = c * kChunk + warp * kTile + t;
+                if (x0 > pos) break;
+                float k[kRow][kCols], v[kRow][kCols];
+#pragma unroll
+                for (int u = 0; u < kRow; ++u) {
+                    const int x = min(x0 + u, pos), n = static_cast<int>(p.page_div.div(x)), page = table[n];
+                    const int64_t at = paged_base(paged_valid(page, pc.num_pages) ? page : 0, kh, pc.kv_heads, pc.page_size, D) +
+                                       static_cast<int64_t>(x - n * pc.page_size) * D + lane;
+#pragma unroll
+                    for (int i = 0; i < kCols; ++i) k[u][i] = to_float(__ldcg(kp + at + 32 * i)), v[u][i] = to_float(__ldcg(vp + at + 32 * i));
+                }
+#pragma unroll
+                for (int u = 0; u < kRow; ++u) {
+                    if (x0 + u > pos) break;
+                    float s[kHeads];
+#pragma unroll
+                    for (int h = 0; h < kHeads; ++h) {
+                        s[h] = 0.0f;
+#pragma unroll
+                        for (int i = 0; i < kCols; ++i) s[h] = fmaf(q[h][i], k[u][i], s[h]);
+                    }
+#pragma unroll
+                    for (int h = 0; h < kHeads; ++h) {
+                        s[h] = warp_sum(s[h]) * (kLog2e / (D == 64 ? 8.0f : 11.313708498984761f));
+                        const bool out = s[h] == -INFINITY;
+                        const float high = fmaxf(top[h], s[h]), old = top[h] == -INFINITY ? 0.0f : exp2_fast(top[h] - high);
+                        const float w = out ? 0.0f : exp2_fast(s[h] - high);
+                        top[h] = high, sum[h] = sum[h] * old + w;
+#pragma unroll
+                        for (int i = 0; i < kCols; ++i) {
+                            const bool finite = fabsf(v[u][i]) < INFINITY;
+                            o[h][i] = o[h][i] * old + (finite ? w * v[u][i] : 0.0f);
+                            if (!finite) past[h][i] += out ? __int_as_float(0x7fffffff) : v[u][i];
+                        }
+                    }
+                }
+            }
+        }
+#pragma unroll
+        for (int h = 0; h < kHeads; ++h) {
+            float* row = part + min(r0 + h, nh - 1) * (D + 2);
+#pragma unroll
+            for (int i = 0; i < kCols; ++i) row[lane + 32 * i] = o[h][i] + past[h][i];
+            if (lane == 0) row[D] = top[h], row[D + 1] = bad ? __int_as_float(0x7fffffff) : sum[h];
+        }
+    }
+}
+
+// A partial output under its factor; an infinite one stays so where the factor is below the floats' range.
+__device__ __forceinline__ float under(float f, float o) { return fabsf(o) == INFINITY ? o : f * o; }
+
 template <typename C, int D, bool WIDE>
-__global__ void __launch_bounds__(128, (AttnShape<C, D, WIDE>::kCtas)) attn_decode_paged_kernel(const AttnParams p) {
+__global__ void __launch_bounds__(128, (AttnShape<C, D, WIDE>::kCtas))
+    attn_decode_paged_kernel(const __grid_constant__ AttnParams p) {
     using S = AttnShape<C, D, WIDE>;
     extern __shared__ __align__(16) float smem[];
     uint4* frag = reinterpret_cast<uint4*>(smem);  // [steps][halves][32]: the queries in the MMA's layout, hi and lo
     float* warp_part = smem;                       // [warps][rows][D + 2], once the queries are no longer read
     __shared__ int flag;
     __shared__ uint32_t row_max[16];
+    __shared__ Stretch held_back;
     const PagedCache& pc = p.pc;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
     const int pairs = pc.kv_heads * p.blocks;  // of a sequence
@@ -308,11 +401,11 @@ __global__ void __launch_bounds__(128, (AttnShape<C, D, WIDE>::kCtas)) attn_deco
             }
         }
     }
-    const long long grid = min(static_cast<long long>(gridDim.x), all);  // a unit at least for every CTA that works
+    long long grid = min(static_cast<long long>(gridDim.x), all);  // a unit at least for every CTA that works
     if (blockIdx.x >= grid) return;
-    const bool brief = paged_brief(all);
+    bool brief = paged_brief(all);
     long long at = paged_share(blockIdx.x, all, grid, brief);
-    const long long end = paged_share(blockIdx.x + 1, all, grid, brief);
+    long long end = paged_share(blockIdx.x + 1, all, grid, brief);
     int b = 0;
     long long first = 0;  // the row's index of sequence b's first unit
     for (int b0 = 0; b0 < pc.batch; b0 += 32) {
@@ -342,7 +435,6 @@ __global__ void __launch_bounds__(128, (AttnShape<C, D, WIDE>::kCtas)) attn_deco
         const int c0 = u0 * step, c1 = min(nch, u1 * step);
         const int kh = pair / p.blocks, blk = pair - kh * p.blocks;
         const int h0 = kh * p.group + blk * S::kRows, nh = min(S::kRows, p.group - blk * S::kRows);
-        const int64_t out0 = (static_cast<int64_t>(b) * p.heads + h0) * D;
         const long long pair_first = first + static_cast<long long>(pair) * nu;
         const int seq = b;
         at += u1 - u0;
@@ -352,6 +444,7 @@ __global__ void __launch_bounds__(128, (AttnShape<C, D, WIDE>::kCtas)) attn_deco
         }
         if (!paged_pos_ok(pos, pc.max_pages, pc.page_size, limit)) {
             const float v = pos == -1 ? 0.0f : __int_as_float(0x7fffffff);
+            const int64_t out0 = (static_cast<int64_t>(seq) * p.heads + h0) * D;
             for (int i = threadIdx.x; i < nh * D; i += 128) store_io(p.out, out0 + i, v, p.io);
             continue;
         }
@@ -479,6 +572,8 @@ __global__ void __launch_bounds__(128, (AttnShape<C, D, WIDE>::kCtas)) attn_deco
             kp[new_at] = from_float<C>(new_row[0]), kp[new_at + D / 2] = from_float<C>(new_row[1]);
             vp[new_at] = from_float<C>(new_row[2]), vp[new_at + D / 2] = from_float<C>(new_row[3]);
         }
+        if (threadIdx.x == 0)
+            held_back = Stretch{at, end, first, all, grid, pair_first, b, step, seq, pos, kh, h0, nh, c0, c1, nch, nu, pair};
         __syncthreads();  // queries, and the new rows, are there for every warp
         if (!early) {
             load_k(rows);
@@ -634,12 +729,28 @@ __global__ void __launch_bounds__(128, (AttnShape<C, D, WIDE>::kCtas)) attn_deco
         }
 
         __syncthreads();  // the queries have been read
+        const Stretch now = held_back;
+        at = now.at, end = now.end, first = now.first, all = now.all, grid = now.grid, b = now.b, step = now.step;
+        brief = paged_brief(all);
+        const int64_t out0 = (static_cast<int64_t>(now.seq) * p.heads + now.h0) * D;
         // The warps' rows: output parts, then maximum and sum.
         bad = __any_sync(0xffffffffu, bad);
+        float odd[4] = {0.0f, 0.0f, 0.0f, 0.0f};  // NaN where a sum is not finite
+#pragma unroll
+        for (int h = 0; h < S::kHalves; ++h)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                odd[j] = fmaf(sum[h][j & 1], 0.0f, odd[j]);
+#pragma unroll
+                for (int i = 0; i < D / 16; ++i) odd[j] = fmaf(acc[h][i][j], 0.0f, odd[j]);
+            }
+        const bool again = __any_sync(0xffffffffu, (odd[0] + odd[1]) + (odd[2] + odd[3]) != 0.0f);
+        if (again) plain_part<C, D>(p, now.seq, now.kh, now.h0, now.nh, now.pos, now.c0, now.c1, bad, warp_part + warp * S::kRows * (D + 2));
 #pragma unroll
         for (int h = 0; h < S::kHalves; ++h)
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
+                if (again) break;
                 float l = sum[h][j];
 #pragma unroll
                 for (int o = 4; o < 32; o <<= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
@@ -654,10 +765,10 @@ __global__ void __launch_bounds__(128, (AttnShape<C, D, WIDE>::kCtas)) attn_deco
                 if (g == 0) row[D] = top[h][j], row[D + 1] = l;
             }
         __syncthreads();
-        const bool whole = c0 == 0 && c1 == nch;
-        const int slot = 2 * blockIdx.x + (c0 > 0 ? 0 : 1);
+        const bool whole = now.c0 == 0 && now.c1 == now.nch;
+        const int slot = 2 * blockIdx.x + (now.c0 > 0 ? 0 : 1);
         float* mine = p.part + slot * static_cast<int64_t>(S::kRows * (D + 2));
-        for (int i = threadIdx.x; i < nh * D; i += 128) {
+        for (int i = threadIdx.x; i < now.nh * D; i += 128) {
             const int r = i / D, d = i - r * D;
             const float* row = warp_part + r * (D + 2);
             float m = -INFINITY, l = 0.0f, o = 0.0f;
@@ -667,7 +778,7 @@ __global__ void __launch_bounds__(128, (AttnShape<C, D, WIDE>::kCtas)) attn_deco
             for (int w = 0; w < kAttnWarps; ++w) {
                 const float* x = row + w * S::kRows * (D + 2);
                 const float f = x[D] == -INFINITY ? 0.0f : exp2f(x[D] - m);
-                l += f * x[D + 1], o += f * x[d];
+                l += f * x[D + 1], o += under(f, x[d]);
                 if (x[D + 1] != x[D + 1]) l = x[D + 1];
             }
             if (whole) {
@@ -680,8 +791,8 @@ __global__ void __launch_bounds__(128, (AttnShape<C, D, WIDE>::kCtas)) attn_deco
         if (whole) continue;
 
         // The pair's last CTA to come here merges all its partials, in CTA order.
-        const int cta0 = paged_owner(pair_first, all, grid, brief), cta1 = paged_owner(pair_first + nu - 1, all, grid, brief);
-        int* ticket = p.tickets + static_cast<int64_t>(seq) * pairs + pair;
+        const int cta0 = paged_owner(now.pair_first, all, grid, brief), cta1 = paged_owner(now.pair_first + now.nu - 1, all, grid, brief);
+        int* ticket = p.tickets + static_cast<int64_t>(now.seq) * pairs + now.pair;
         __syncthreads();  // the partial is written; one thread's fence carries it to the others' reads
         if (threadIdx.x == 0) {
             __threadfence();
@@ -693,7 +804,7 @@ __global__ void __launch_bounds__(128, (AttnShape<C, D, WIDE>::kCtas)) attn_deco
         // A warp a head, 4 columns a lane (d = 64: half a warp takes every other partial), kMergeAhead partials in
         // flight: a long sequence alone has dozens of them, and one at a time would cost a memory round trip each.
         constexpr int kLanes = D / 4, kApart = 32 / kLanes;
-        for (int r = warp; r < nh; r += kAttnWarps) {
+        for (int r = warp; r < now.nh; r += kAttnWarps) {
             float m = -INFINITY, l = 0.0f, o[4] = {0.0f, 0.0f, 0.0f, 0.0f};
             const int d = (lane % kLanes) * 4;
             for (int c = cta0; c <= cta1; c += kMergeAhead * kApart) {
@@ -716,8 +827,8 @@ __global__ void __launch_bounds__(128, (AttnShape<C, D, WIDE>::kCtas)) attn_deco
                     const float f0 = m == -INFINITY ? 0.0f : exp2_fast(m - up);
                     const float f1 = ml[k].x == -INFINITY ? 0.0f : exp2_fast(ml[k].x - up);
                     l = ml[k].y != ml[k].y ? ml[k].y : l * f0 + ml[k].y * f1;
-                    o[0] = o[0] * f0 + x[k][0].x * f1, o[1] = o[1] * f0 + x[k][0].y * f1;
-                    o[2] = o[2] * f0 + x[k][1].x * f1, o[3] = o[3] * f0 + x[k][1].y * f1;
+                    o[0] = under(f0, o[0]) + under(f1, x[k][0].x), o[1] = under(f0, o[1]) + under(f1, x[k][0].y);
+                    o[2] = under(f0, o[2]) + under(f1, x[k][1].x), o[3] = under(f0, o[3]) + under(f1, x[k][1].y);
                     m = up;
                 }
             }
@@ -727,7 +838,7 @@ __global__ void __launch_bounds__(128, (AttnShape<C, D, WIDE>::kCtas)) attn_deco
                 const float f0 = m == -INFINITY ? 0.0f : exp2_fast(m - up), f1 = m2 == -INFINITY ? 0.0f : exp2_fast(m2 - up);
                 l = l != l || l2 != l2 ? __int_as_float(0x7fffffff) : l * f0 + l2 * f1;
 #pragma unroll
-                for (int k = 0; k < 4; ++k) o[k] = o[k] * f0 + __shfl_xor_sync(0xffffffffu, o[k], 16) * f1;
+                for (int k = 0; k < 4; ++k) o[k] = under(f0, o[k]) + under(f1, __shfl_xor_sync(0xffffffffu, o[k], 16));
             }
             if (lane < kLanes) {
 #pragma unroll
