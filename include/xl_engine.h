@@ -394,7 +394,9 @@ XL_API int xl_op_add_rmsnorm_fp8(int dtype, const void* delta, const void* resid
  * [n][ceil(k / 128)], wq [m][k] with w_scale [ceil(m / 128)][ceil(k / 128)];
  * sums in fp32.  The modes of xl_op_linear: 0 y [n][m]; 1 SwiGLU over
  * interleaved (W1, V) rows, y [n][m / 2], m even; 2 y [n][m] += .  dtype is
- * y's type; bias [m] may be NULL. */
+ * y's type; bias [m] may be NULL.  The kernels wait for their own copies and
+ * products 0.2 s at most: outputs whose wait ran out (a GPU given to another
+ * program meanwhile) are NaN, with no status. */
 XL_API int xl_op_linear_fp8(int mode, int dtype, const uint8_t* xq, size_t ldx, const float* x_scale, const uint8_t* wq,
                             size_t ldw, const float* w_scale, const float* bias, void* y, int n, int m, int k,
                             void* stream);

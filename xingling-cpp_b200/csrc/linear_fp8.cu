@@ -29,6 +29,7 @@
 #include <algorithm>
 #include <atomic>
 
+#include "drain.h"
 #include "fp8.cuh"
 #include "tcgen05.cuh"
 #include "xl_device.cuh"
@@ -317,8 +318,8 @@ __global__ void __launch_bounds__(Pair::kThreads, 1)
     uint64_t* full = reinterpret_cast<uint64_t*>(reinterpret_cast<char*>(store) + Pair::kStoreBytes);
     uint64_t* empty = full + kMaxStages;
     uint64_t* done = empty + kMaxStages;   // an accumulator holds a K-block's sums
-    uint64_t* freed = done + Pair::kAccs;  // its columns have been read, in both CTAs
-    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(freed + Pair::kAccs);
+    uint64_t* freed = done + Pair::kAccs;  // its columns have been read, in both CTAs (see DrainTurn for their number)
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(freed + 2 * Pair::kAccs);
 
     const int warp = __shfl_sync(0xffffffffu, static_cast<int>(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
     const int rank = static_cast<int>(cluster_rank());
@@ -331,10 +332,8 @@ __global__ void __launch_bounds__(Pair::kThreads, 1)
             mbar_init(&full[lane], 1);
             mbar_init(&empty[lane], 1);
         }
-        if (lane < Pair::kAccs) {
-            mbar_init(&done[lane], 1);
-            mbar_init(&freed[lane], 2 * Pair::kEpiWarps);
-        }
+        if (lane < Pair::kAccs) mbar_init(&done[lane], 1);
+        if (lane < 2 * Pair::kAccs) mbar_init(&freed[lane], 2 * Pair::kEpiWarps);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if (warp == 1) {
@@ -388,7 +387,7 @@ __global__ void __launch_bounds__(Pair::kThreads, 1)
         if (rank == 0) {
             int s = 0, a = 0;
             uint32_t ph = 0, pa = 0;
-            bool ok = true;
+            bool ok = true, any = false;
             for (int t = unit; t < tiles && ok; t += units) {
                 for (int kb = 0; kb < p.blocks; ++kb) {
                     if (!wait_warp(&full[s], ph) || !wait_warp(&freed[a], pa ^ 1u)) {
@@ -407,9 +406,14 @@ __global__ void __launch_bounds__(Pair::kThreads, 1)
                         commit<2>(&empty[s]);
                     }
                     __syncwarp();
+                    any = true;
                     if (++s == p.stages) s = 0, ph ^= 1u;
                     if (++a == Pair::kAccs) a = 0, pa ^= 1u;
                 }
+            }
+            if (!ok && any) {  // the MMAs in flight end before the TMEM is given back
+                if (a == 0) a = Pair::kAccs, pa ^= 1u;
+                wait_warp(&done[a - 1], pa);
             }
         }
     } else if (warp >= Pair::kEpiFirst) {
@@ -418,9 +422,7 @@ __global__ void __launch_bounds__(Pair::kThreads, 1)
         const int q = warp & 3, half = (warp - Pair::kEpiFirst) >> 2;
         float* st = store + (warp - Pair::kEpiFirst) * Pair::kWarpStore;
         float* sb = st + 32 * kStagePitch;
-        int a = 0;
-        uint32_t pa = 0;
-        bool ok = true;
+        DrainTurn<Pair::kAccs> turn;
         const uint32_t freed0 = cluster_addr(smem_u32(freed), 0);
         for (int t = unit; t < tiles; t += units) {
             const int tok0 = t % p.tiles_n * Pair::kTokens + rank * 128 + 32 * q;
@@ -438,20 +440,21 @@ __global__ void __launch_bounds__(Pair::kThreads, 1)
 #pragma unroll
             for (int i = 0; i < 64; ++i) acc[i] = 0;
             float sx = xs[0], sw = ws[0];
-            bool ready = mbar_test_wait(&done[a], pa);
+            bool ready = mbar_test_wait(&done[turn.acc], turn.parity);
 #pragma unroll 1
             for (int kb = 0; kb < p.blocks; ++kb) {
                 const float s = sx * sw;
                 const int next = min(kb + 1, p.blocks - 1);
                 sx = xs[next], sw = ws[next];
-                if (ok && !__all_sync(0xffffffffu, ready)) ok = wait_warp(&done[a], pa);
+                if (turn.ok && !__all_sync(0xffffffffu, ready))
+                    turn.waited(wait_warp(&done[turn.acc], turn.parity));
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                const bool drain = work && ok;
+                const bool drain = work && turn.ok;
                 const unsigned long long s2 = pack2(__float_as_uint(s), __float_as_uint(s));
                 uint32_t r0[32], r1[32];
                 if (drain) {
                     const uint32_t ta = tmem + (static_cast<uint32_t>(32 * q) << 16) +
-                                        static_cast<uint32_t>(a * Pair::kFeatures + 128 * half);
+                                        static_cast<uint32_t>(turn.acc * Pair::kFeatures + 128 * half);
                     // two rounds of 64 columns in flight; the accumulator is handed back before the last sums
                     tmem_load32(ta, r0);
                     tmem_load32(ta + 32, r1);
@@ -467,15 +470,15 @@ __global__ void __launch_bounds__(Pair::kThreads, 1)
                 if (elect_one())
                     // only TMEM reads are ordered by this arrival (the fence above); a cluster-wide release of
                     // memory would cost over 1000 clocks a K-block
-                    asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(freed0 + 8 * a) : "memory");
-                if (++a == Pair::kAccs) a = 0, pa ^= 1u;
-                if (kb + 1 < p.blocks) ready = mbar_test_wait(&done[a], pa);  // asked early: the answer comes behind the sums
+                    asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(freed0 + 8 * turn.acc) : "memory");
+                turn.next();
+                if (kb + 1 < p.blocks) ready = mbar_test_wait(&done[turn.acc], turn.parity);  // asked early: the answer comes behind the sums
                 if (drain) {
                     scale_in(acc, 32, r0, s2);
                     scale_in(acc, 48, r1, s2);
                 }
             }
-            if (!ok) {  // a wait ran out: the results say so
+            if (!turn.ok) {  // a wait ran out: the results say so
 #pragma unroll
                 for (int i = 0; i < 64; ++i) acc[i] = 0x7fffffff7fffffffull;
             }
@@ -591,7 +594,8 @@ __global__ void __launch_bounds__(Few<N>::kThreads, Few<N>::kCtas)
     uint64_t* empty = full + kMaxStages;
     uint64_t* done = empty + kMaxStages;
     uint64_t* freed = done + F::kAccs;
-    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(freed + F::kAccs);
+    uint64_t* quiet = freed + 2 * F::kAccs;  // both issuing warps have stopped
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(quiet + 1);
 
     const int warp = __shfl_sync(0xffffffffu, static_cast<int>(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
     const uint32_t rank = p.split > 1 ? cluster_rank() : 0u;
@@ -606,10 +610,9 @@ __global__ void __launch_bounds__(Few<N>::kThreads, Few<N>::kCtas)
             mbar_init(&full[lane], 1);
             mbar_init(&empty[lane], 1);
         }
-        if (lane < F::kAccs) {
-            mbar_init(&done[lane], 1);
-            mbar_init(&freed[lane], 4);
-        }
+        if (lane < F::kAccs) mbar_init(&done[lane], 1);
+        if (lane < 2 * F::kAccs) mbar_init(&freed[lane], 4);
+        if (lane == 0) mbar_init(quiet, 2);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if (warp == 1) {
@@ -653,10 +656,12 @@ __global__ void __launch_bounds__(Few<N>::kThreads, Few<N>::kCtas)
                 wait_warp(&full[s], ph);
             }
         }
+        __syncwarp();
+        if (elect_one()) asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(quiet)) : "memory");
     } else if (warp == 1) {
         int s = 0, a = 0;
         uint32_t ph = 0, pa = 0;
-        bool ok = true;
+        bool ok = true, any = false;
         for (int t = unit; t < tiles && ok; t += units) {
             for (int kb = kb0; kb < kb1; ++kb) {
                 if (!wait_warp(&freed[a], pa ^ 1u) || !wait_warp(&full[s], ph)) {
@@ -674,16 +679,21 @@ __global__ void __launch_bounds__(Few<N>::kThreads, Few<N>::kCtas)
                     commit<1>(&done[a]);
                 }
                 __syncwarp();
+                any = true;
                 if (++s == p.stages) s = 0, ph ^= 1u;
                 if (++a == F::kAccs) a = 0, pa ^= 1u;
             }
         }
+        if (!ok && any) {  // the MMAs in flight end before the TMEM is given back
+            if (a == 0) a = F::kAccs, pa ^= 1u;
+            wait_warp(&done[a - 1], pa);
+        }
+        __syncwarp();
+        if (elect_one()) asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(quiet)) : "memory");
     } else {
         const int q = warp & 3;
         float* sc = scales + (warp - 2) * N;
-        int a = 0;
-        uint32_t pa = 0;
-        bool ok = true;
+        DrainTurn<F::kAccs> turn;
         constexpr int kLots = (N + 31) / 32;
         for (int t = unit; t < tiles; t += units) {
             const int tok0 = t % p.tiles_n * N, tm = t / p.tiles_n, rows = min(N, p.n - tok0);
@@ -699,7 +709,7 @@ __global__ void __launch_bounds__(Few<N>::kThreads, Few<N>::kCtas)
             float sx[kLots], sw = ws[kb0];
 #pragma unroll
             for (int i = 0; i < kLots; ++i) sx[i] = xs[i][kb0];
-            bool ready = mbar_test_wait(&done[a], pa);
+            bool ready = mbar_test_wait(&done[turn.acc], turn.parity);
 #pragma unroll 1
             for (int kb = kb0; kb < kb1; ++kb) {
 #pragma unroll
@@ -710,13 +720,14 @@ __global__ void __launch_bounds__(Few<N>::kThreads, Few<N>::kCtas)
 #pragma unroll
                 for (int i = 0; i < kLots; ++i) sx[i] = xs[i][next];
                 __syncwarp();
-                if (ok && !__all_sync(0xffffffffu, ready)) ok = wait_warp(&done[a], pa);
+                if (turn.ok && !__all_sync(0xffffffffu, ready))
+                    turn.waited(wait_warp(&done[turn.acc], turn.parity));
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                 uint32_t r[F::kRound];
-                const uint32_t ta = tmem + (static_cast<uint32_t>(32 * q) << 16) + static_cast<uint32_t>(a * N);
+                const uint32_t ta = tmem + (static_cast<uint32_t>(32 * q) << 16) + static_cast<uint32_t>(turn.acc * N);
 #pragma unroll
                 for (int c = 0; c < N; c += F::kRound) {
-                    if (ok) {
+                    if (turn.ok) {
 #pragma unroll
                         for (int i = 0; i < F::kRound; i += 16) tmem_load16(ta + c + i, r + i);
 #pragma unroll
@@ -726,11 +737,11 @@ __global__ void __launch_bounds__(Few<N>::kThreads, Few<N>::kCtas)
                         asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
                         __syncwarp();
                         if (elect_one())
-                            asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(&freed[a])) : "memory");
-                        if (++a == F::kAccs) a = 0, pa ^= 1u;
-                        if (kb + 1 < kb1) ready = mbar_test_wait(&done[a], pa);
+                            asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(&freed[turn.acc])) : "memory");
+                        turn.next();
+                        if (kb + 1 < kb1) ready = mbar_test_wait(&done[turn.acc], turn.parity);
                     }
-                    if (ok) {
+                    if (turn.ok) {
 #pragma unroll
                         for (int i = 0; i < F::kRound / 4; ++i) {
                             const ulonglong2 s4 = reinterpret_cast<const ulonglong2*>(sc)[c / 4 + i];
@@ -741,7 +752,7 @@ __global__ void __launch_bounds__(Few<N>::kThreads, Few<N>::kCtas)
                 }
                 __syncwarp();
             }
-            if (!ok) {  // a wait ran out: the results say so
+            if (!turn.ok) {  // a wait ran out: the results say so
 #pragma unroll
                 for (int i = 0; i < N / 2; ++i) acc[i] = 0x7fffffff7fffffffull;
             }
@@ -773,7 +784,10 @@ __global__ void __launch_bounds__(Few<N>::kThreads, Few<N>::kCtas)
                     }
                 }
             } else {
-                // every K-block of this CTA has been multiplied: the ring is free for the partial tile [tokens][128]
+                // every K-block of this CTA has been multiplied: the ring is free for the partial tile [tokens][128]; where a
+                // wait ran out, only once the issuing warps have stopped and their copies have landed
+                for (int i = 0; i < 8 && !turn.ok; ++i)
+                    if (wait_warp(quiet, 0)) break;
                 float* part = reinterpret_cast<float*>(ring);
 #pragma unroll
                 for (int i = 0; i < N; ++i) {

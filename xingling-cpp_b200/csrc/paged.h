@@ -3,11 +3,7 @@
 #pragma once
 #include <stdint.h>
 
-#ifdef __CUDACC__
-#define XL_HD __host__ __device__ __forceinline__
-#else
-#define XL_HD inline
-#endif
+#include "xl_hd.h"
 
 namespace xl {
 
