@@ -231,3 +231,25 @@ def test_attend_infinite_query(torch):
         assert torch.equal(bad, want)
         for b in range(2):
             check(torch, p, dq, None, b, n, out, heads)
+
+
+# ---- the product -----------------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("n", [3, 12, 20, 100, 1100])
+def test_linear_swiglu_of_large_negative_gates(torch, n):
+    """silu(v) is v e^v to the end of the floats' range: gates of -60 to -91.5, where e^-v passes it, times 2^60."""
+    m, k = 2602, 130
+    g = T.gen(torch, n)
+    dx, dw = (torch.zeros((r, T.pitch(k)), dtype=torch.uint8, device="cuda") for r in (n, m))
+    xs, ws = torch.zeros((n, 2), device="cuda"), torch.zeros(((m + 127) // 128, 2), device="cuda")
+    bias = torch.empty(m)
+    bias[0::2] = -(60 + 31.5 * torch.rand(m // 2, generator=g))
+    bias[1::2] = 2.0 ** 60
+    y = torch.empty((n, m // 2), device="cuda")
+    db = bias.cuda()
+    X.check(X.lib().xl_op_linear_fp8(1, 0, X.ptr(dx), dx.stride(0), X.ptr(xs), X.ptr(dw), dw.stride(0), X.ptr(ws), X.ptr(db),
+                                     X.ptr(y), n, m, k, X.stream()))
+    v = bias[0::2].double()
+    want = (v * torch.sigmoid(v) * bias[1::2].double()).expand(n, -1)
+    off = (y.cpu().double() - want).abs() / want.abs()
+    assert float(off.max()) <= 16 * U, float(off.max())

@@ -181,7 +181,14 @@ __device__ __forceinline__ void scale_in(unsigned long long (&acc)[64], int firs
     for (int i = 0; i < 16; ++i) fma2(acc[first + i], pack2(r[2 * i], r[2 * i + 1]), s2);
 }
 
-__device__ __forceinline__ float silu_fast(float v) { return __fdividef(v, 1.0f + expf(-v)); }  // within 5 ulp
+// v / (1 + e^-v) = v e^v / (1 + e^v), within 7 ulp.  With e^-|v| as the square of h = e^(-|v| / 2) no step leaves the
+// floats' range before the result does (e^-v passes it at v = -89, where v e^v has not, and the fast division gives 0 for
+// divisors above 2^126); without a branch, of which a tile's store would hold one an output (13.6 us of a 512 x 8192 x 1536
+// product became 16.9).
+__device__ __forceinline__ float silu_fast(float v) {
+    const float h = expf(-0.5f * fabsf(v)), e = h * h;
+    return __fdividef(v < 0.0f ? v * h * h : v, 1.0f + e);
+}
 
 template <typename T>
 __device__ __forceinline__ void put(T* dst, float v, int mode) {
