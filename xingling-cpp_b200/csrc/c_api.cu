@@ -2,7 +2,6 @@
 #include <cuda.h>
 #include <nccl.h>
 
-#include <atomic>
 #include <cstring>
 #include <initializer_list>
 #include <string>
@@ -10,6 +9,7 @@
 
 #include "engine.h"
 #include "paged.h"
+#include "per_device.h"
 
 using xl::Engine;
 
@@ -487,10 +487,9 @@ PointerAttributeFn pointer_attribute() {
 }
 
 int on_current_device(const char* what, std::initializer_list<const void*> ptrs, int* sms) {
-    constexpr int kDevices = 64;
-    static std::atomic<int> sm_count[kDevices];  // 0: not asked yet
+    static xl::PerDevice sm_count;
     int dev = 0;
-    int rc = cuda_status(cudaGetDevice(&dev), what);
+    const int rc = cuda_status(cudaGetDevice(&dev), what);
     if (rc != XL_OK) return rc;
     const PointerAttributeFn attribute = pointer_attribute();
     if (!attribute) return cuda_status(cudaErrorNotSupported, what);
@@ -503,14 +502,13 @@ int on_current_device(const char* what, std::initializer_list<const void*> ptrs,
             return XL_ERR_ARG;
         }
     }
-    const int known = dev < kDevices ? sm_count[dev].load(std::memory_order_relaxed) : 0;
-    if (known) {
-        *sms = known;
-        return XL_OK;
-    }
-    rc = cuda_status(cudaDeviceGetAttribute(sms, cudaDevAttrMultiProcessorCount, dev), what);
-    if (rc == XL_OK && dev < kDevices) sm_count[dev].store(*sms, std::memory_order_relaxed);
-    return rc;
+    cudaError_t e = cudaSuccess;
+    *sms = sm_count.get(dev, [&] {
+        int n = 0;
+        e = cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev);
+        return n;
+    });
+    return cuda_status(e, what);
 }
 
 // Null if the cache's description is in order, else what is wrong with it.

@@ -31,6 +31,7 @@
 
 #include "drain.h"
 #include "fp8.cuh"
+#include "per_device.h"
 #include "tcgen05.cuh"
 #include "xl_device.cuh"
 #include "xl_kernels.h"
@@ -983,11 +984,10 @@ cudaError_t launch_stream(const StreamParams& p, int num_sms, cudaStream_t s) {
 
 int cdiv(long long a, long long b) { return static_cast<int>((a + b - 1) / b); }
 
-// Clusters of `split` CTAs that the GPU runs at once with a CTA an SM (asked once a size).
+// Clusters of `split` CTAs that the current device runs at once with a CTA an SM.
 template <typename Kernel>
-int clusters_at_once(Kernel kernel, std::atomic<int>& known, int split, int threads) {
-    int n = known.load(std::memory_order_relaxed);
-    if (n) return n;
+int clusters_at_once(Kernel kernel, int split, int threads) {
+    int n = 0;
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3(static_cast<unsigned>(split));
     cfg.blockDim = dim3(static_cast<unsigned>(threads));
@@ -1003,19 +1003,23 @@ int clusters_at_once(Kernel kernel, std::atomic<int>& known, int split, int thre
         cudaGetLastError();
         return 0;
     }
-    known.store(n, std::memory_order_relaxed);
     return n;
 }
 
 // K split over how many CTAs: as many as run at once, powers of two.
 template <int N, typename T>
 int few_split(long long tiles, int blocks, int num_sms) {
-    static std::atomic<int> known[4];  // clusters of 2, 4, 8
+    static PerDevice at_once[3];  // clusters of 2, 4, 8
+    auto clusters = [&](int i, int s) {
+        int dev = -1;
+        if (cudaGetDevice(&dev) != cudaSuccess) return 0;
+        return at_once[i].get(dev, [&] { return clusters_at_once(linear_fp8_few_kernel<N, T>, s, Few<N>::kThreads); });
+    };
     int split = 1;
     for (int i = 0, s = 2; s <= kMaxSplit && s <= blocks; ++i, s *= 2) {
         // two CTAs an SM (fewer stages, see below) leave room to place the clusters of one wave of CTAs
         const bool fits = Few<N>::kCtas > 1 ? tiles * s <= num_sms
-                                            : tiles <= clusters_at_once(linear_fp8_few_kernel<N, T>, known[i], s, Few<N>::kThreads);
+                                            : tiles <= clusters(i, s);
         if (!fits) break;
         split = s;
     }
