@@ -253,3 +253,47 @@ def test_linear_swiglu_of_large_negative_gates(torch, n):
     want = (v * torch.sigmoid(v) * bias[1::2].double()).expand(n, -1)
     off = (y.cpu().double() - want).abs() / want.abs()
     assert float(off.max()) <= 16 * U, float(off.max())
+
+
+# ---- the norm --------------------------------------------------------------------------------------------------------
+
+def near_ties(torch, groups, t, seed):
+    """r, gamma of one row whose groups each hold two largest products that round to one fp32 number and differ: the
+    larger comes second, a few lanes on, in the same lane, or at the group's end."""
+    g = T.gen(torch, seed)
+    r = (torch.randn(groups * 128, generator=g) * 0.05).to(t)
+    gamma = torch.rand(groups * 128, generator=g) * 0.5 + 0.5
+    for i in range(groups):
+        first, second = i * 128 + 8 * (i % 13) + 1, i * 128 + [8 * (i % 13) + 5, 8 * (i % 13) + 20, 127][i % 3]
+        while True:
+            a, b = ((torch.rand(2, generator=g) + 1) * 2).to(t)
+            wa = torch.rand((), generator=g) + 1
+            product = (a.double() * wa.double())
+            wb = (product / b.double()).float()
+            for _ in range(2):
+                exact = b.double() * wb.double()
+                if exact > product and exact.float() == product.float():
+                    break
+                wb = torch.nextafter(wb, torch.tensor(math.inf))
+            else:
+                continue
+            break
+        r[first], gamma[first], r[second], gamma[second] = a, wa, b, wb
+    return r, gamma
+
+
+@pytest.mark.parametrize("dtype", [0, 1, 2], ids=["fp32", "bf16", "fp16"])
+@pytest.mark.parametrize("groups,n", [(8, 1), (64, 3), (64, 400), (250, 2)])
+def test_norm_scale_of_tied_products(torch, dtype, groups, n):
+    """The scale is made of the largest exact product, also where another one rounds to the same fp32 number."""
+    t, k = T.types(torch)[dtype], groups * 128
+    r, gamma = near_ties(torch, groups, t, groups + dtype)
+    res = (r.float() * 2.0 ** torch.arange(n).remainder(5)[:, None]).to(t)  # powers of two keep the ties
+    d_res, d_gamma = res.cuda(), gamma.cuda()
+    q, s = torch.empty((n, k), dtype=torch.uint8, device="cuda"), torch.empty((n, groups), device="cuda")
+    X.check(X.lib().xl_op_add_rmsnorm_fp8(dtype, None, X.ptr(d_res), None, X.ptr(d_gamma), X.ptr(q), k, X.ptr(s), n, k,
+                                          X.stream()))
+    some = list(range(min(n, 5)))
+    _, (want_q, want_s) = T.norm_reference(torch, None, res[some], gamma)
+    T.same(torch, s[some], want_s)
+    T.same(torch, q[some].view(torch.float8_e4m3fn), want_q)

@@ -185,8 +185,9 @@ __device__ __forceinline__ double inverse_root(double v) {
 // 1 / sqrt(mean(r^2) + eps), y = r gamma rs, e4m3 per row and 128 columns.
 // One row a CTA, kept in registers (CHUNKS x 8 columns a thread), so each
 // input is read once.  The sum of squares is 64-bit and the largest |r gamma|
-// of a group is taken with the remainder of its fp32 product (rounding keeps
-// the order), so that a group's scale is the rounded exact one.  fp32 rows are
+// of a group is taken with the remainder of its fp32 product, the largest among
+// those that round to the same (rounding keeps the order, but not strictly), so
+// that a group's scale is the rounded exact one.  fp32 rows are
 // bound by their bytes (4095 x 8192: 75 us, 5.8 TB/s), bf16 rows by some 35
 // instructions a value (60 us, 4.0 TB/s); 8 x 1536 takes 2.4 us, a row's chain.
 template <typename T, int CHUNKS, int THREADS, bool VEC>
@@ -255,24 +256,26 @@ __global__ void __launch_bounds__(THREADS, THREADS == 256 ? 3 : 1) add_rmsnorm_f
         const int live = max(0, min(8, k - c));
         float w[8], p[8];
         to_floats(load_raw8<VEC>(gamma + (live ? c : 0), live), w);
-        float own = 0.0f, own_r = 0.0f, own_w = 0.0f;  // the lane's largest product (NaN if there is one), its factors
+        float own = 0.0f;  // the lane's largest product (NaN if there is one)
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
             p[i] = r[j][i] * w[i];
-            const float size = fabsf(p[i]);
-            const bool up = size > own;
-            own_r = up ? r[j][i] : own_r, own_w = up ? w[i] : own_w;
-            asm("max.NaN.f32 %0, %0, %1;" : "+f"(own) : "f"(size));
+            asm("max.NaN.f32 %0, %0, %1;" : "+f"(own) : "f"(fabsf(p[i])));
         }
         const uint32_t mine = __float_as_uint(own);
         uint32_t a = mine;
 #pragma unroll
         for (int o = kLanesPerGroup / 2; o; o >>= 1) a = umax(a, __shfl_xor_sync(0xffffffffu, a, o));
-        // the group's largest product, exactly: its rounded value and the remainder
-        const uint32_t holders = __ballot_sync(0xffffffffu, mine == a) & (0xffffu << (threadIdx.x & 16));
-        const int holder = __ffs(holders) - 1;
-        const float wr = __shfl_sync(0xffffffffu, own_r, holder), ww = __shfl_sync(0xffffffffu, own_w, holder);
-        const float top = __uint_as_float(a), rest = fmaf(fabsf(wr), fabsf(ww), -top);
+        // the group's largest product, exactly: its rounded value and the largest remainder among those that round to it
+        const float top = __uint_as_float(a);
+        float rest = -INFINITY;
+        if (mine == a) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                if (fabsf(p[i]) == top) rest = fmaxf(rest, fmaf(fabsf(r[j][i]), fabsf(w[i]), -top));
+        }
+#pragma unroll
+        for (int o = kLanesPerGroup / 2; o; o >>= 1) rest = fmaxf(rest, __shfl_xor_sync(0xffffffffu, rest, o));
         // top / 448 / root to 2^-46, then rounded once
         const float t = top * rs_hi;
         float s = t + (fmaf(top, rs_hi, -t) + fmaf(top, rs_lo, rest * rs_hi));
