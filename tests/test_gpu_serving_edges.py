@@ -2,6 +2,7 @@
 scores far apart, infinities and NaN in the cache, batches whose work crosses
 sequences, ties, and the ends of the floats' range.  The bounds are those of
 test_gpu_serving_ops.py, whose helpers are used."""
+import ctypes as C
 import math
 
 import pytest
@@ -233,7 +234,106 @@ def test_attend_infinite_query(torch):
             check(torch, p, dq, None, b, n, out, heads)
 
 
+def chunks(pos):
+    return [n // 64 + 1 if n >= 0 else 1 for n in pos]
+
+
+LONG = [
+    # dtype, cache, batch, heads, kv, d, page, longest
+    (1, 1, 70, 32, 8, 128, 64, 4000),
+    (0, 2, 70, 32, 8, 64, 24, 3000),
+    (2, 2, 66, 64, 4, 128, 32, 5000),
+    (0, 0, 70, 26, 2, 64, 100, 6000),
+    (0, 0, 45, 20, 4, 128, 16, 3000),
+    (0, 1, 130, 64, 4, 64, 16, 2500),
+]
+
+
+@pytest.mark.parametrize("dtype,cache,batch,heads,kv,d,page,longest", LONG)
+def test_attend_many_long_sequences(torch, dtype, cache, batch, heads, kv, d, page, longest):
+    """More than eight chunks a CTA: stretches cross heads and sequences, and each warp's loop runs long.  Slots without
+    a sequence and positions out of range lie among them."""
+    t = T.types(torch)[dtype]
+    g = T.gen(torch, batch + d)
+    pos = [max(0, int(longest * (i + 1) / batch) - 1) for i in torch.randperm(batch, generator=g).tolist()]
+    pos[3], pos[40] = -1, -1
+    blocks = (heads // kv + 15) // 16 if heads // kv > 8 else 1
+    grid = torch.cuda.get_device_properties(0).multi_processor_count * 3
+    assert sum(chunks(pos)) * kv * blocks > 8 * grid
+    p = Pool(torch, cache, [n + 1 for n in pos], kv, d, page, seed=batch)
+    rope = T.rope_table(torch, longest + 1, d).cuda()
+    given = list(pos)
+    given[7], given[35] = -9, longest + 100  # no position of this cache
+    d_pos = torch.tensor(given, dtype=torch.int32, device="cuda")
+    ws, outs = T.workspace(torch, p.c, heads), []
+    qkv = torch.randn((batch, (heads + 2 * kv) * d), generator=g).to(t).cuda()
+    for _ in range(2):
+        out = torch.full((batch + 1, heads * d), 5.0, dtype=t, device="cuda")
+        T.attend(torch, p, dtype, qkv, rope, d_pos, out, heads, ws)
+        outs.append(out)
+    assert (out[batch] == 5).all() and (out[[3, 40]] == 0).all() and out[[7, 35]].isnan().all()
+    as_int = torch.int32 if t == torch.float32 else torch.int16
+    assert torch.equal(outs[0].view(as_int), outs[1].view(as_int))
+    for b in sorted(set(range(0, batch, 5)) | {0, 1, 31, 32, 33, batch - 1}):
+        if b not in (3, 7, 35, 40):
+            check(torch, p, qkv, rope, b, pos[b], out, heads)
+
+
+@CACHES
+@pytest.mark.parametrize("batch,heads,kv,d", [(60, 16, 8, 64), (33, 64, 16, 128), (200, 24, 4, 64)])
+def test_attend_more_pairs_than_ctas(torch, cache, batch, heads, kv, d):
+    """More pairs than CTAs but few chunks: single chunks are cut across pairs and sequences."""
+    g = T.gen(torch, batch)
+    pos = [int(x) for x in torch.randint(0, 64, (batch,), generator=g)]
+    pos[1], pos[batch - 2], pos[batch // 2] = 700, 300, -1
+    grid = torch.cuda.get_device_properties(0).multi_processor_count * 3
+    assert grid < sum(chunks(pos)) * kv < 8 * grid and batch * kv > grid
+    p = Pool(torch, cache, [n + 1 for n in pos], kv, d, 16, seed=batch)
+    rope = T.rope_table(torch, 701, d).cuda()
+    d_pos = torch.tensor(pos, dtype=torch.int32, device="cuda")
+    qkv = torch.randn((batch, (heads + 2 * kv) * d), generator=g).cuda()
+    ws, outs = T.workspace(torch, p.c, heads), []
+    for _ in range(2):
+        out = torch.empty((batch, heads * d), device="cuda")
+        T.attend(torch, p, 0, qkv, rope, d_pos, out, heads, ws)
+        outs.append(out)
+    assert torch.equal(*outs)
+    for b, n in enumerate(pos):
+        if n < 0:
+            assert (out[b] == 0).all()
+        else:
+            check(torch, p, qkv, rope, b, n, out, heads)
+
+
 # ---- the product -----------------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("dtype", [0, 1, 2], ids=["fp32", "bf16", "fp16"])
+@pytest.mark.parametrize("n,m,k", [(9, 130, 129), (12, 514, 2050), (16, 1000, 1536), (16, 20010, 300), (5, 40002, 272),
+                                   (10, 256, 4096), (1, 80002, 130), (15, 600, 513)])
+def test_linear_up_to_16_tokens(torch, dtype, n, m, k):
+    """Features on the TMEM lanes with 16 token columns: K whole and split over 2, 4 and 8 CTAs, partial tiles."""
+    T.test_linear(torch, dtype, n, m, k)
+
+
+def test_linear_on_several_streams_against_64_bits(torch):
+    """Calls of different shapes under way together, each held to its 64-bit form."""
+    cases = []
+    for i, (n, m, k) in enumerate([(8, 4608, 1536), (16, 1536, 4096), (32, 4608, 1536), (64, 1536, 4096), (100, 1536, 1536),
+                                   (300, 4608, 1536), (12, 512, 2048)]):
+        g = T.gen(torch, i + 50)
+        (dx, x), (dw, w) = T.random_fp8(torch, n, k, g), T.random_fp8(torch, m, k, g)
+        xs, ws = torch.rand((n, k // 128), generator=g), torch.rand((m // 128, k // 128), generator=g) * 1e-3
+        cases.append((n, m, k, dx, dw, xs.cuda(), ws.cuda(), torch.empty((n, m), device="cuda"), torch.cuda.Stream(), x, w))
+    torch.cuda.synchronize()
+    for _ in range(20):
+        for n, m, k, dx, dw, xs, ws, y, stream, _, _ in cases:
+            X.check(X.lib().xl_op_linear_fp8(0, 0, X.ptr(dx), dx.stride(0), X.ptr(xs), X.ptr(dw), dw.stride(0), X.ptr(ws), None,
+                                             X.ptr(y), n, m, k, C.c_void_p(stream.cuda_stream)))
+    torch.cuda.synchronize()
+    for n, m, k, dx, dw, xs, ws, y, stream, x, w in cases:
+        want, bound = T.linear_reference(torch, 0, x, xs.cpu(), w, ws.cpu(), None, None)
+        assert ((y.cpu().double() - want).abs() <= bound + U * want.abs()).all(), (n, m, k)
+
 
 @pytest.mark.parametrize("n", [3, 12, 20, 100, 1100])
 def test_linear_swiglu_of_large_negative_gates(torch, n):
