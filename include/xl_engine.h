@@ -439,9 +439,9 @@ XL_API int xl_op_kv_append_paged(const xl_paged_kv* cache, int dtype, const void
  * as the cache holds them (scale head_dim^-1/2).  heads is a multiple of
  * kv_heads; query head h reads key/value head h / (heads / kv_heads).
  * Statistics and sums are fp32; queries and weights meet a bf16 cache with 16
- * bits (2^-17 relative), an fp16 one with 22 (what is below 2^-28 of the largest
- * weight, or of the query's largest element, with 2^-51 of that), an fp32 one
- * with 21 to 22.  Infinities and NaN in the cache count as the formula says: a
+ * bits (2^-17 relative; all 24 of them where the rows are fp32), an fp16 one with
+ * 22 (what is below 2^-28 of the largest weight, or of the query's largest
+ * element, with 2^-51 of that), an fp32 one with 21 to 22.  Infinities and NaN in the cache count as the formula says: a
  * score of minus infinity is a weight of 0, an infinite value an infinite output,
  * a score of infinity or NaN, 0 x inf and inf - inf NaN.
  * pos[b] = -1: no sequence, zeros.  Any other position out of range, or a page

@@ -132,6 +132,30 @@ def test_attend_queries_of_uneven_size(torch):
     check(torch, p, dq, None, 0, n, out, heads)
 
 
+@CACHES
+@pytest.mark.parametrize("heads,kv,d", [(4, 2, 64), (8, 1, 128), (12, 1, 64), (32, 2, 128)])
+def test_attend_fp32_rows_keep_their_bits(torch, cache, heads, kv, d):
+    """Two positions, one element of the query that counts: out = 1 / (1 + e^-s) of a 24-bit s.  Nothing is summed but
+    the query's parts (4 steps of 2u), the scale takes 4u more and the split 2^-21 at most; the rest as in the other
+    bound."""
+    batch = 64
+    p = Pool(torch, cache, [2] * batch, kv, d, 4, seed=3)
+    p.k.zero_()
+    p.v.zero_()
+    g = T.gen(torch, heads + d)
+    qkv = torch.zeros((batch, heads + 2 * kv, d))
+    qkv[:, :heads, 0] = (torch.rand((batch, heads), generator=g) * 40 - 20) * math.sqrt(d)
+    qkv[:, heads:heads + kv, 0], qkv[:, heads + kv:] = 1.0, 1.0
+    dq, out = qkv.view(batch, -1).cuda(), torch.empty((batch, heads * d), device="cuda")
+    pos = torch.ones(batch, dtype=torch.int32, device="cuda")
+    T.attend(torch, p, 0, dq, None, pos, out, heads, T.workspace(torch, p.c, heads))
+    s = qkv[:, :heads, 0].double() / math.sqrt(d)
+    want = torch.sigmoid(s)
+    tol = (2 * (12 * U + 2.0 ** -21) * s.abs() + 2.0 ** -21 + 18 * 2 * U + 2.0 ** -20) * want
+    off = (out.view(batch, heads, d).cpu().double() - want[..., None]).abs() - (tol + U * want)[..., None]
+    assert (off <= 0).all(), float((off / want[..., None]).max())
+
+
 def special(torch, p, rows, b, n, what, heads):
     """Makes sequence b (last position n) hold `what`; element 0 of every query is -1, element 1 is 4 sqrt(d)."""
     kv, d, mid = p.kv, p.d, n // 2

@@ -4,6 +4,7 @@
 #include <math.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "fp8.cuh"
 #include "paged.h"
@@ -96,7 +97,8 @@ __global__ void __launch_bounds__(kAppendThreads) kv_append_paged_kernel(const P
 //
 // Precision: queries are split in two 16-bit halves, and so are the weights,
 // which leaves 2^-17 (bf16) or 2^-23 (fp16) of error where rounding them would
-// leave 2^-9 or 2^-12; an fp32 cache runs as three TF32 products of split
+// leave 2^-9 or 2^-12; fp32 rows over a bf16 cache take three parts, which are
+// all of an fp32 value; an fp32 cache runs as three TF32 products of split
 // operands.  fp16 has no value below 2^-24 and none above 65504: what is split
 // for it is scaled by powers of two, the low half by one more, so that a weight
 // keeps its 2^-23 down to 2^-29 of the largest (e^-20) and an absolute 2^-52
@@ -176,6 +178,14 @@ __device__ __forceinline__ uint4 load_shared(const uint4* p) {
     return v;
 }
 
+__device__ __forceinline__ uint2 load_shared(const uint2* p) {
+    uint2 v;
+    asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];"
+                 : "=r"(v.x), "=r"(v.y)
+                 : "r"(static_cast<uint32_t>(__cvta_generic_to_shared(p))));
+    return v;
+}
+
 // fp16 holds 5 exponent bits: a query row is scaled by 2^-row_exponent so that its largest value is in [2^14, 2^15), which
 // leaves an element 2^-28 of that its 2^-23.  (A row below 2^-112 is scaled by less; its scores are zeros beside 1.)
 template <typename C>
@@ -193,6 +203,13 @@ constexpr float kLowUp = kScaled<C> ? 4096.0f : 1.0f;
 // What the weights (at most 1) are scaled by: up to 2^15 is below fp16's largest value.
 template <typename C>
 constexpr float kWeightUp = kScaled<C> ? 32768.0f : 1.0f;
+
+// What two bf16 halves leave of two values: with it they have 24 bits, fp32's own.
+__device__ __forceinline__ uint32_t rest16(float a, float b, uint32_t hi, uint32_t lo) {
+    const float2 h = make_float2(__uint_as_float(hi << 16), __uint_as_float(hi & 0xffff0000u));
+    const float2 l = make_float2(__uint_as_float(lo << 16), __uint_as_float(lo & 0xffff0000u));
+    return pack_pair((a - h.x) - l.x, (b - h.y) - l.y, __nv_bfloat16{});
+}
 
 // Two values as a pair of 16-bit halves: v = hi + lo / kLowUp up to 2^-17 (bf16) or 2^-23 (fp16, from 2^-14 on) of it.
 template <typename C>
@@ -248,7 +265,8 @@ __device__ __forceinline__ float exp2_fast(float v) {  // 2^-22 relative, 0 belo
 __device__ __forceinline__ uint32_t word(const uint4& v, int i) { return i == 0 ? v.x : i == 1 ? v.y : i == 2 ? v.z : v.w; }
 
 // C: cache type, D: head dim, WIDE: 16 query heads a pair (else 8), as two column halves of the MMAs.
-template <typename C, int D, bool WIDE>
+// PARTS: 16-bit values that a query or weight is split into.
+template <typename C, int D, bool WIDE, int PARTS>
 struct AttnShape {
     static constexpr bool k32 = sizeof(C) == 4;
     static constexpr int kVec = 16 / sizeof(C);             // elements of a 16-byte load
@@ -258,7 +276,7 @@ struct AttnShape {
     static constexpr int kHalves = WIDE ? 2 : 1;
     static constexpr int kRows = 8 * kHalves;
     static constexpr int kPer = kVec / 2;                   // columns of a lane in a step
-    static constexpr int kFragFloats = kSteps * kHalves * 128;
+    static constexpr int kFragFloats = kSteps * kHalves * (PARTS == 3 ? 192 : 128);
     static constexpr int kPartFloats = kAttnWarps * kRows * (D + 2);
     static constexpr int kSmemFloats = kFragFloats > kPartFloats ? kFragFloats : kPartFloats;
     // CTAs an SM holds, by registers: a lane keeps a tile's keys and values and its part of the output
@@ -357,12 +375,13 @@ __device__ __forceinline__ void plain_part(const AttnParams& p, int seq, int kh,
 // A partial output under its factor; an infinite one stays so where the factor is below the floats' range.
 __device__ __forceinline__ float under(float f, float o) { return fabsf(o) == INFINITY ? o : f * o; }
 
-template <typename C, int D, bool WIDE>
-__global__ void __launch_bounds__(128, (AttnShape<C, D, WIDE>::kCtas))
+template <typename C, int D, bool WIDE, int PARTS>
+__global__ void __launch_bounds__(128, (AttnShape<C, D, WIDE, PARTS>::kCtas))
     attn_decode_paged_kernel(const __grid_constant__ AttnParams p) {
-    using S = AttnShape<C, D, WIDE>;
+    using S = AttnShape<C, D, WIDE, PARTS>;
     extern __shared__ __align__(16) float smem[];
     uint4* frag = reinterpret_cast<uint4*>(smem);  // [steps][halves][32]: the queries in the MMA's layout, hi and lo
+    uint2* frag3 = reinterpret_cast<uint2*>(frag + S::kSteps * S::kHalves * 32);  // their third parts, where there are such
     float* warp_part = smem;                       // [warps][rows][D + 2], once the queries are no longer read
     __shared__ int flag;
     __shared__ uint32_t row_max[16];
@@ -562,9 +581,15 @@ __global__ void __launch_bounds__(128, (AttnShape<C, D, WIDE>::kCtas))
                 split16<C>(qa[n][0] * down, qa[n][1] * down, o.x, o.z);
                 split16<C>(qa[n][S::kPer - 2] * down, qa[n][S::kPer - 1] * down, o.y, o.w);
                 *fa = o;
+                if constexpr (PARTS == 3)
+                    frag3[fa - frag] = make_uint2(rest16(qa[n][0], qa[n][1], o.x, o.z),
+                                                  rest16(qa[n][S::kPer - 2], qa[n][S::kPer - 1], o.y, o.w));
                 split16<C>(qb[n][0] * down, qb[n][1] * down, o.x, o.z);
                 split16<C>(qb[n][S::kPer - 2] * down, qb[n][S::kPer - 1] * down, o.y, o.w);
                 *fb = o;
+                if constexpr (PARTS == 3)
+                    frag3[fb - frag] = make_uint2(rest16(qb[n][0], qb[n][1], o.x, o.z),
+                                                  rest16(qb[n][S::kPer - 2], qb[n][S::kPer - 1], o.y, o.w));
             }
         }
         if (new_at >= 0) {
@@ -628,6 +653,10 @@ __global__ void __launch_bounds__(128, (AttnShape<C, D, WIDE>::kCtas))
                         mma_tf32(more[h], lo, q.x, q.y);
                     } else {
                         mma16(large, a, q.x, q.y, C{});
+                        if constexpr (PARTS == 3) {
+                            const uint2 q3 = load_shared(frag3 + (i * S::kHalves + h) * 32 + lane);
+                            mma16(more[h], a, q3.x, q3.y, C{});
+                        }
                         mma16(more[h], a, q.z, q.w, C{});
                     }
                 }
@@ -669,7 +698,7 @@ __global__ void __launch_bounds__(128, (AttnShape<C, D, WIDE>::kCtas))
                         for (int j = 0; j < 4; ++j) acc[h][i][j] *= old[h][j & 1];
             }
             // The weights as the next MMAs' second operand: head g, positions 2t, 2t + 1 and those + 8.
-            uint32_t wh[S::kHalves][4], wl[S::kHalves][4];
+            uint32_t wh[S::kHalves][4], wl[S::kHalves][4], w3[S::kHalves][2];
 #pragma unroll
             for (int h = 0; h < S::kHalves; ++h)
 #pragma unroll
@@ -684,6 +713,7 @@ __global__ void __launch_bounds__(128, (AttnShape<C, D, WIDE>::kCtas))
                         uint32_t hi, lo;
                         split16<C>(s[h][2 * n] * kWeightUp<C>, s[h][2 * n + 1] * kWeightUp<C>, hi, lo);
                         wh[h][n] = transpose8(hi), wl[h][n] = transpose8(lo);
+                        if constexpr (PARTS == 3) w3[h][n] = transpose8(rest16(s[h][2 * n], s[h][2 * n + 1], hi, lo));
                     }
                 }
 #pragma unroll
@@ -716,6 +746,7 @@ __global__ void __launch_bounds__(128, (AttnShape<C, D, WIDE>::kCtas))
                                            __byte_perm(z, u, 0x7632)};
 #pragma unroll
                     for (int h = 0; h < S::kHalves; ++h) {
+                        if constexpr (PARTS == 3) mma16(o[h], a, w3[h][0], w3[h][1], C{});
                         mma16(kScaled<C> ? low[h] : o[h], a, wl[h][0], wl[h][1], C{});
                         mma16(o[h], a, wh[h][0], wh[h][1], C{});
                     }
@@ -862,15 +893,19 @@ cudaError_t append_typed(const PagedCache& pc, const void* qkv, const float* rop
     return cudaGetLastError();
 }
 
-template <typename C, int D, bool WIDE>
+template <typename C, int D, bool WIDE, int PARTS = 2>
 cudaError_t attend_shape(AttnParams p, int num_sms, cudaStream_t s) {
-    using S = AttnShape<C, D, WIDE>;
+    // fp32 rows over a bf16 cache take a third part: 64 sequences up to 8192, 32 heads on 8: 194 us and 2.5e-7 of the output
+    // off, where two parts take 181 and leave 3.2e-6. The rounding of 16-bit rows (1.7e-3) hides that: 186 us against 192.
+    if constexpr (std::is_same_v<C, __nv_bfloat16> && PARTS == 2)
+        if (p.io == kF32) return attend_shape<C, D, WIDE, 3>(p, num_sms, s);
+    using S = AttnShape<C, D, WIDE, PARTS>;
     p.blocks = (p.group - 1) / S::kRows + 1;
     const long long longest = static_cast<long long>(p.pc.max_pages) * p.pc.page_size;
     const long long chunks = ((longest - 1) / kChunk + 1) * p.pc.batch * p.pc.kv_heads * p.blocks;
     const long long most = std::min(num_sms * S::kCtas, kPagedMaxCtas);
     count_launch();
-    attn_decode_paged_kernel<C, D, WIDE>
+    attn_decode_paged_kernel<C, D, WIDE, PARTS>
         <<<static_cast<int>(std::min(chunks, most)), 128, S::kSmemFloats * sizeof(float), s>>>(p);
     return cudaGetLastError();
 }
