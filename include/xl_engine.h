@@ -424,8 +424,11 @@ typedef struct xl_paged_kv {
 /* Keys and values of `rows` rows (prompts) into their pages: row i of qkv
  * ([rows][(heads + 2 kv_heads) head_dim], q | k | v) goes to position
  * row_pos[i] of sequence row_seq[i] (device ints), its key rotated by the
- * angles rope[row_pos[i]] ([rope_len][head_dim / 2] pairs of cos and sin:
- * xl_rope_table for head_dim 64) or as it is where rope is NULL.  A row whose
+ * angles rope[row_pos[i]] ([rope_len][head_dim / 2] pairs (c, s) of cos and sin:
+ * xl_rope_table for head_dim 64) or as it is where rope is NULL.  The rotation
+ * is the engine's: elements a = x[j] and b = x[j + head_dim / 2] become
+ * a c + b s and b c - a s, by minus the angle (a host whose keys are turned the
+ * other way passes -sin); queries below are turned alike.  A row whose
  * sequence, position or page is out of range is skipped; positions past
  * rope_len are out of range.  No two rows may name one position (what is
  * stored there is then a mixture of theirs). */
