@@ -104,8 +104,8 @@ __global__ void __launch_bounds__(kAppendThreads) kv_append_paged_kernel(const P
 // keeps its 2^-23 down to 2^-29 of the largest (e^-20) and an absolute 2^-52
 // below.  Sums, maxima and the running output are fp32.
 //
-// 64 sequences up to 8192 (32 heads on 8 of 128, bf16): 202 us, 5.4 TB/s; one
-// of 131072: 101 us, 5.3 TB/s.  8 sequences up to 768 (24 heads of 64, fp32):
+// 64 sequences up to 8192 (32 heads on 8 of 128, bf16): 187 us, 5.8 TB/s; one
+// of 131072: 96 us, 5.6 TB/s.  8 sequences up to 768 (24 heads of 64, fp32):
 // 16 us, of which reading the cache would be 6.4; the rest is the chain of one
 // stretch: finding it 1.6, first loads 2, merging 2.
 
@@ -280,7 +280,9 @@ struct AttnShape {
     static constexpr int kPartFloats = kAttnWarps * kRows * (D + 2);
     static constexpr int kSmemFloats = kFragFloats > kPartFloats ? kFragFloats : kPartFloats;
     // CTAs an SM holds, by registers: a lane keeps a tile's keys and values and its part of the output
-    // (4 and 5, with spills: 212 and 306 us where 3 takes 194, 64 sequences up to 8192 in bf16)
+    // (4 and 5, with spills throughout, took 212 and 306 us where 3 took 194, 64 sequences up to 8192 in bf16).
+    // What spills as it is, in bytes stored: an fp32 cache with 9 to 16 heads a pair, 68 at width 128 and 40
+    // at 64; 8 or none elsewhere.
     static constexpr int kCtas = D == 128 && (k32 || WIDE) ? 2 : 3;
 };
 

@@ -131,8 +131,10 @@ __global__ void __launch_bounds__(256) quantize_rows_kernel(const T* __restrict_
 
 // One scale per block of 128 x 128: a CTA keeps the block in registers, so it
 // is read once (64 values a thread, 16 loads of 16 bytes in flight for fp32).
-// Bound by its bytes: 151669 x 1536 fp32 in 197 us, 5.9 TB/s.  bf16 blocks meet
-// exact borders often and are bound by their arithmetic (26620 x 2072: 87 us).
+// Bound by its bytes: 151669 x 1536 fp32 in 197 us, 5.9 TB/s.  bf16 blocks are
+// not (26620 x 2072: 87 us, 1.9 TB/s): 8-bit values meet exact borders often and
+// a warp then takes the 64-bit path, though borders decided by a remainder's
+// sign instead took as long, so that may not be all of it.
 template <typename T, bool VEC>
 __global__ void __launch_bounds__(256) quantize_blocks_kernel(const T* __restrict__ x, size_t ldx, uint8_t* __restrict__ q,
                                                               size_t ldq, float* __restrict__ scale, FastDiv per_row,
@@ -188,8 +190,8 @@ __device__ __forceinline__ double inverse_root(double v) {
 // of a group is taken with the remainder of its fp32 product, the largest among
 // those that round to the same (rounding keeps the order, but not strictly), so
 // that a group's scale is the rounded exact one.  fp32 rows are
-// bound by their bytes (4095 x 8192: 75 us, 5.8 TB/s), bf16 rows by some 35
-// instructions a value (60 us, 4.0 TB/s); 8 x 1536 takes 2.4 us, a row's chain.
+// bound by their bytes (4095 x 8192: 77 us, 5.7 TB/s), bf16 rows by some 40
+// instructions a value (60 us, 3.9 TB/s); 8 x 1536 takes 2.4 us, a row's chain.
 template <typename T, int CHUNKS, int THREADS, bool VEC>
 __global__ void __launch_bounds__(THREADS, THREADS == 256 ? 3 : 1) add_rmsnorm_fp8_kernel(const T* __restrict__ delta, const T* residual, T* sum,
                                                                   const float* __restrict__ gamma,
