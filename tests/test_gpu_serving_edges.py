@@ -329,6 +329,37 @@ def test_attend_more_pairs_than_ctas(torch, cache, batch, heads, kv, d):
             check(torch, p, qkv, rope, b, n, out, heads)
 
 
+def test_attend_on_two_streams_at_once(torch):
+    """Two captured calls, each with a workspace of its own, replayed together many times: each holds to its 64-bit form,
+    and every replay gives the same bits."""
+    sides = []
+    for i, (cache, batch, heads, kv, d, n) in enumerate([(1, 40, 32, 8, 128, 900), (2, 70, 12, 4, 64, 300)]):
+        pos = [max(0, n * (b + 1) // batch - 1) for b in range(batch)]
+        p = Pool(torch, cache, [x + 1 for x in pos], kv, d, 16, seed=i)
+        if i:
+            p.put("v", 5, 0, math.inf)
+        qkv = torch.randn((batch, (heads + 2 * kv) * d), generator=T.gen(torch, i)).cuda()
+        out, dp = torch.empty((batch, heads * d), device="cuda"), torch.tensor(pos, dtype=torch.int32, device="cuda")
+        ws, stream, graph = T.workspace(torch, p.c, heads), torch.cuda.Stream(), torch.cuda.CUDAGraph()
+        torch.cuda.synchronize()
+        with torch.cuda.graph(graph, stream=stream):
+            for _ in range(5):
+                T.attend(torch, p, 0, qkv, None, dp, out, heads, ws, stream=stream)
+        sides.append((p, qkv, pos, out, heads, ws, stream, graph, dp))
+    first = None
+    for _ in range(10):
+        for side in sides:
+            with torch.cuda.stream(side[6]):
+                side[7].replay()
+        torch.cuda.synchronize()
+        now = [side[3].view(torch.int32).clone() for side in sides]
+        first = first or now
+        assert all(torch.equal(a, b) for a, b in zip(first, now))
+    for p, qkv, pos, out, heads, *_ in sides:
+        for b, n in enumerate(pos):
+            check(torch, p, qkv, None, b, n, out, heads)
+
+
 # ---- the product -----------------------------------------------------------------------------------------------------
 
 @pytest.mark.parametrize("dtype", [0, 1, 2], ids=["fp32", "bf16", "fp16"])
